@@ -201,6 +201,144 @@ def int8_conv_transpose2d_k2s2_forward(input, weight, w_scale, bias):
     return out
 
 
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # FORGE_DTYPE_*
+_BYTES_PER_BLOCK = 64   # packed 4-bit weights: 128 inputs
+
+
+def _act_dtype(x):
+    """FORGE_DTYPE_* of a 2-D fp16 / bf16 activation whose row length the kernels take."""
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"x: expected torch.float16 or torch.bfloat16, got {x.dtype}")
+    if x.dim() != 2 or x.size(1) == 0 or x.size(1) % 8 != 0:
+        raise ValueError(f"x: expected (tokens, inputs) with inputs a positive multiple of 8, got {tuple(x.shape)}")
+    return _DTYPES[x.dtype]
+
+
+def _shape(**named):
+    for name, (t, shape) in named.items():
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+
+
+def _aligned(t):
+    """`t` at a 16-byte aligned address (a view into a larger buffer may start anywhere)."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_group(group_size):
+    if group_size not in (32, 64, 128):
+        raise ValueError(f"group_size: expected 32, 64 or 128, got {group_size}")
+
+
+def prepare_weight_int4(weight, group_size=128):
+    """Float weight (N, K) on a GPU -> (w_int4 uint8 (N, ceil(K / 128) * 64), w_scale fp16 (ceil(K / group_size), N)):
+    4-bit integers in the layout of include/forge_b200.h with one scale per group of 32, 64 or 128 inputs."""
+    if weight.dtype not in _DTYPES:
+        weight = weight.to(torch.float32)
+    weight = weight.contiguous()
+    _chk(weight)
+    _check_group(group_size)
+    if weight.dim() != 2 or weight.size(1) == 0 or weight.size(1) % 8 != 0:
+        raise ValueError(f"weight: expected (outputs, inputs) with inputs a positive multiple of 8, got {tuple(weight.shape)}")
+    weight = _aligned(weight)
+    N, K = weight.shape
+    w_int4 = torch.empty((N, (K + 127) // 128 * _BYTES_PER_BLOCK), dtype=_u8, device=weight.device)
+    w_scale = torch.empty(((K + group_size - 1) // group_size, N), dtype=_f16, device=weight.device)
+    with _on(weight):
+        _lib.call("forge_prepare_weight_int4", _ptr(weight), _DTYPES[weight.dtype], _ptr(w_int4), _ptr(w_scale), N, K,
+                  group_size, _stream())
+    return w_int4, w_scale
+
+
+def _int4_operand(x, name, w, s, b, N, group_size):
+    """Checks one 4-bit weight with its scales and bias against x (M, K) and N outputs."""
+    K = x.size(1)
+    _chk(x, **{name + "_int4": (w, _u8), name + "_scale": (s, _f16), "bias of " + name: (b, x.dtype)})
+    _shape(**{name + "_int4": (w, (N, (K + 127) // 128 * _BYTES_PER_BLOCK)),
+              name + "_scale": (s, ((K + group_size - 1) // group_size, N)), "bias of " + name: (b, (N,))})
+    if w.data_ptr() % 16 != 0:
+        raise ValueError(f"{name}_int4: must start at a 16-byte aligned address")
+
+
+def int4_linear(x, w_int4, w_scale, bias=None, group_size=128):
+    """x (M, K) fp16 / bf16 times a 4-bit weight (prepare_weight_int4) plus bias (N) of x's type -> (M, N)."""
+    dtype = _act_dtype(x)
+    _check_group(group_size)
+    _chk(x, x=(x, x.dtype))
+    M, K = x.shape
+    N = w_int4.size(0)
+    _int4_operand(x, "w", w_int4, w_scale, bias, N, group_size)
+    x = _aligned(x)
+    output = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    with _on(x):
+        _lib.call("forge_int4_linear", _ptr(x), _ptr(w_int4), _ptr(w_scale), _ptr(bias), _ptr(output), M, K, N,
+                  group_size, dtype, _stream())
+    return output
+
+
+def int4_gated_linear(x, wg_int4, wu_int4, wg_scale, wu_scale, bg=None, bu=None, group_size=128):
+    """SiLU(x Wg^T + bg) * (x Wu^T + bu) for 4-bit weights, one kernel -> (M, N)."""
+    dtype = _act_dtype(x)
+    _check_group(group_size)
+    _chk(x, x=(x, x.dtype))
+    M, K = x.shape
+    N = wg_int4.size(0)
+    _int4_operand(x, "wg", wg_int4, wg_scale, bg, N, group_size)
+    _int4_operand(x, "wu", wu_int4, wu_scale, bu, N, group_size)
+    x = _aligned(x)
+    output = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    with _on(x):
+        _lib.call("forge_int4_gated_linear", _ptr(x), _ptr(wg_int4), _ptr(wu_int4), _ptr(wg_scale), _ptr(wu_scale),
+                  _ptr(bg), _ptr(bu), _ptr(output), M, K, N, group_size, dtype, _stream())
+    return output
+
+
+def gated_linear(x, Wg, Wu, bg=None, bu=None, save=False):
+    """SiLU(x Wg^T + bg) * (x Wu^T + bu) for fp16 / bf16 weights (N, K) -> (M, N). save=True: also the two products in
+    fp32, (h, g, u), which gated_linear_backward takes. No autograd; see forge_b200.nn.gated_linear."""
+    dtype = _act_dtype(x)
+    M, K = x.shape
+    N = Wg.size(0)
+    _chk(x, x=(x, x.dtype), Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), bg=(bg, x.dtype), bu=(bu, x.dtype))
+    _shape(Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), bg=(bg, (N,)), bu=(bu, (N,)))
+    if N % 8 != 0:
+        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, got {N}")
+    x, Wg, Wu = _aligned(x), _aligned(Wg), _aligned(Wu)
+    h = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    g = u = None
+    if save:
+        g = torch.empty((M, N), dtype=_f32, device=x.device)
+        u = torch.empty((M, N), dtype=_f32, device=x.device)
+    with _on(x):
+        _lib.call("forge_gated_linear", _ptr(x), _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), _ptr(h), _ptr(g), _ptr(u), M, K,
+                  N, dtype, _stream())
+    return (h, g, u) if save else h
+
+
+def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=True):
+    """Gradients of gated_linear for dh (M, N): (dx, dWg, dWu, dbg, dbu) in x's type, None where not asked for."""
+    dtype = _act_dtype(x)
+    M, K = x.shape
+    N = Wg.size(0)
+    _chk(x, dh=(dh, x.dtype), x=(x, x.dtype), Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), g=(g, _f32), u=(u, _f32))
+    _shape(dh=(dh, (M, N)), Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), g=(g, (M, N)), u=(u, (M, N)))
+    if N % 8 != 0:
+        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, got {N}")
+    # without tokens the library writes nothing, and the gradients of the weights are zero
+    new = torch.zeros if M == 0 else torch.empty
+    dx = new((M, K), dtype=x.dtype, device=x.device) if need_x else None
+    dWg, dWu = (new((N, K), dtype=x.dtype, device=x.device) if need_w else None for _ in range(2))
+    dbg, dbu = (new((N,), dtype=x.dtype, device=x.device) if need_b else None for _ in range(2))
+    dh, x, Wg, Wu = _aligned(dh), _aligned(x), _aligned(Wg), _aligned(Wu)
+    g, u = _aligned(g), _aligned(u)
+    with _on(x):
+        size = _lib.load().forge_gated_linear_backward_workspace_bytes(M, N)
+        workspace = torch.empty((size,), dtype=_u8, device=x.device)
+        _lib.call("forge_gated_linear_backward", _ptr(dh), _ptr(x), _ptr(Wg), _ptr(Wu), _ptr(g), _ptr(u), _ptr(dx),
+                  _ptr(dWg), _ptr(dWu), _ptr(dbg), _ptr(dbu), M, K, N, dtype, _ptr(workspace), _stream())
+    return dx, dWg, dWu, dbg, dbu
+
+
 def device_status(reset=True):
     """FORGE_B200_OK (0) unless a kernel on the current device gave up on a bounded wait since the last
     reset (then FORGE_B200_DEVICE_TIMEOUT, 5); `device_status_raw` returns the recorded code."""

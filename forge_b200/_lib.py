@@ -38,6 +38,12 @@ SIGNATURES = {
     "forge_w8a8_gated_mlp_workspace_bytes": [_i, _i, _i],
     "forge_w8a8_gated_mlp": [_vp] * 11 + [_i, _i, _i, _vp, _vp],
     "forge_sparse_w8a8_gated_mlp": [_vp] * 14 + [_i, _i, _i, _vp, _vp],
+    "forge_gated_linear": [_vp] * 8 + [_i] * 4 + [_vp],
+    "forge_gated_linear_backward_workspace_bytes": [_i, _i],
+    "forge_gated_linear_backward": [_vp] * 11 + [_i] * 4 + [_vp, _vp],
+    "forge_prepare_weight_int4": [_vp, _i, _vp, _vp, _i, _i, _i, _vp],
+    "forge_int4_linear": [_vp] * 5 + [_i] * 5 + [_vp],
+    "forge_int4_gated_linear": [_vp] * 8 + [_i] * 5 + [_vp],
     "forge_prune_compress_24": [_vp, _vp, _vp, _i, _i, _vp],
     "forge_pack_metadata": [_vp, _vp, _i, _i, _vp],
     "forge_prepare_weight": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp],
@@ -88,8 +94,8 @@ def load():
             fn.restype = ctypes.c_char_p
         elif name.startswith("forge_b200_probe_"):
             fn.restype = ctypes.c_double
-        elif name in ("forge_w8a8_gated_mlp_workspace_bytes", "forge_int8_conv2d_workspace_size",
-                      "forge_int8_conv_transpose2d_k2s2_workspace_size"):
+        elif name in ("forge_w8a8_gated_mlp_workspace_bytes", "forge_gated_linear_backward_workspace_bytes",
+                      "forge_int8_conv2d_workspace_size", "forge_int8_conv_transpose2d_k2s2_workspace_size"):
             fn.restype = ctypes.c_ulonglong
         else:
             fn.restype = ctypes.c_int

@@ -3,11 +3,14 @@
 #include "../../include/forge_b200.h"
 #include "common.cuh"
 #include "conv.cuh"
+#include "gated_linear.cuh"
 #include "gemm_dense.cuh"
 #include "gemm_pair.cuh"
 #include "gemm_sparse.cuh"
 #include "gemm_fq.cuh"
+#include "int4.cuh"
 #include "kernels.cuh"
+#include "wstream.cuh"
 
 using namespace fb200;
 
@@ -50,6 +53,9 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, const __half*
     if (bias != nullptr) v += __half2float(bias[i % N_out]);
     out[i] = __float2half_rn(v);
 }
+
+inline bool is_16bit(int dtype) { return dtype == FORGE_DTYPE_F16 || dtype == FORGE_DTYPE_BF16; }
+inline bool is_group(int g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
 
@@ -294,6 +300,74 @@ int forge_sparse_w8a8_gated_mlp(const void* x, const int8_t* Wg_comp, const uint
     const BehindQuantizer dependent;
     return sparse_gemm_dequant(Wd_comp, w.hq, wd_meta, w.hs, H(wd_scale), H(bd), H(out), M, d_ffn, d_model, S(stream),
                                force_sparse_bt());
+}
+
+int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void* bg, const void* bu, void* h,
+                       float* g_out, float* u_out, int M, int K, int N, int dtype, forge_stream_t stream) {
+    if (M <= 0 || K <= 0 || N <= 0) return kOk;
+    if (x == nullptr || Wg == nullptr || Wu == nullptr || h == nullptr || (g_out == nullptr) != (u_out == nullptr))
+        return kBadPointer;
+    if (K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(x) || !aligned16(Wg) || !aligned16(Wu) ||
+        !aligned16(h) || !aligned16(g_out) || !aligned16(u_out))
+        return kBadShape;
+    if (!device_is_sm100()) return kUnsupportedArch;
+    return gated_linear(x, Wg, Wu, bg, bu, h, g_out, u_out, M, K, N, dtype == FORGE_DTYPE_BF16, S(stream));
+}
+
+unsigned long long forge_gated_linear_backward_workspace_bytes(int M, int N) {
+    return M <= 0 || N <= 0 ? 0 : gated_linear_backward_workspace(M, N);
+}
+
+int forge_gated_linear_backward(const void* dh, const void* x, const void* Wg, const void* Wu, const float* g,
+                                const float* u, void* dx, void* dWg, void* dWu, void* dbg, void* dbu, int M, int K,
+                                int N, int dtype, void* workspace, forge_stream_t stream) {
+    if (M <= 0 || K <= 0 || N <= 0) return kOk;
+    if (dh == nullptr || x == nullptr || Wg == nullptr || Wu == nullptr || g == nullptr || u == nullptr ||
+        workspace == nullptr || (dWg == nullptr) != (dWu == nullptr))
+        return kBadPointer;
+    if (K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(dh) || !aligned16(x) || !aligned16(Wg) ||
+        !aligned16(Wu) || !aligned16(g) || !aligned16(u) || !aligned16(dx) || !aligned16(dWg) || !aligned16(dWu) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+        return kBadShape;
+    if (!device_is_sm100()) return kUnsupportedArch;
+    return gated_linear_backward(dh, x, Wg, Wu, g, u, dx, dWg, dWu, dbg, dbu, M, K, N, dtype == FORGE_DTYPE_BF16,
+                                 workspace, S(stream));
+}
+
+int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, void* w_scale, int N, int K,
+                              int group_size, forge_stream_t stream) {
+    if (N <= 0 || K <= 0) return kOk;
+    if (weight == nullptr || w_int4 == nullptr || w_scale == nullptr) return kBadPointer;
+    if (K % 8 != 0 || !is_group(group_size) || dtype < FORGE_DTYPE_F32 || dtype > FORGE_DTYPE_BF16 ||
+        !aligned16(weight) || !aligned16(w_int4))
+        return kBadShape;
+    if (!device_is_sm100()) return kUnsupportedArch;
+    return prepare_weight_int4(weight, dtype, w_int4, H(w_scale), N, K, group_size, S(stream));
+}
+
+int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale, const void* bias, void* output, int M,
+                      int K, int N, int group_size, int dtype, forge_stream_t stream) {
+    if (M <= 0 || K <= 0 || N <= 0) return kOk;
+    if (x == nullptr || w_int4 == nullptr || w_scale == nullptr || output == nullptr) return kBadPointer;
+    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(w_int4)) return kBadShape;
+    if (!device_is_sm100()) return kUnsupportedArch;
+    return wstream(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
+                   dtype == FORGE_DTYPE_BF16, S(stream));
+}
+
+int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t* wu_int4, const void* wg_scale,
+                            const void* wu_scale, const void* bg, const void* bu, void* output, int M, int K, int N,
+                            int group_size, int dtype, forge_stream_t stream) {
+    if (M <= 0 || K <= 0 || N <= 0) return kOk;
+    if (x == nullptr || wg_int4 == nullptr || wu_int4 == nullptr || wg_scale == nullptr || wu_scale == nullptr ||
+        output == nullptr)
+        return kBadPointer;
+    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(wg_int4) ||
+        !aligned16(wu_int4))
+        return kBadShape;
+    if (!device_is_sm100()) return kUnsupportedArch;
+    return wstream(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
+                   dtype == FORGE_DTYPE_BF16, S(stream));
 }
 
 int forge_prune_compress_24(const int8_t* weight, int8_t* compressed, uint8_t* metadata_raw, int N, int K,

@@ -7,10 +7,16 @@ parameters with the same names, dtypes and layouts (`w_int8`, `w_scale`, `bias`;
 the other. Weight quantisation is the reference's recipe (per output channel, absmax / 127,
 round half to even, clamp to +-127, scale stored as fp16).
 
+Without a counterpart there: `Int4Linear` (4-bit weights with group scales, for decoding), `GatedLinear` (the
+gate of a Llama-style MLP on unquantized weights, trainable) and `Int4GatedLinear`, which serves the latter.
+
 Beyond the reference: inputs with more than two dimensions are flattened over the leading
 dimensions, non-contiguous inputs are made contiguous, and `SparseLinear.from_dense_weight`
 prunes on the module's own device instead of assuming "cuda".
 """
+import math
+
+import numpy as np
 import torch
 import torch.nn as nn
 
@@ -134,3 +140,165 @@ class SparseLinear(nn.Module, _ScratchMixin):
     def extra_repr(self):
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.bias is not None}, sparse=2:4")
+
+
+def quantize_weight_int4(weight_fp, group_size=128):
+    """(N, K) float weight -> (w_int4, w_scale) as `_forge_C.prepare_weight_int4` gives them, on any device."""
+    w = weight_fp.detach()
+    if w.is_cuda:
+        return _C.prepare_weight_int4(w, group_size)
+    N, K = w.shape
+    groups = -(-K // group_size)
+    w = torch.nn.functional.pad(w.to(torch.float32).to(torch.float64), (0, groups * group_size - K)).view(N, groups, group_size)
+    with np.errstate(over="ignore"):   # beyond fp16: infinity, which becomes NaN below
+        s = torch.from_numpy((w.abs().amax(2) / 7).numpy().astype(np.float16))   # one rounding
+    s[~torch.isfinite(s)] = float("nan")
+    q = torch.clamp(torch.round(w / s.to(torch.float64)[:, :, None]), -7, 7)
+    q[~(s > 0)] = 0
+    q = torch.nn.functional.pad(q.to(torch.int64).view(N, -1)[:, :K], (0, -K % 128)) + 8
+    # blocks of 128: run 4j + t of eight weights is word 4t + j; weight 2i in nibble i, weight 2i + 1 in nibble i + 4
+    q = q.view(N, -1, 4, 4, 4, 2).transpose(2, 3).transpose(4, 5).reshape(N, -1, 2)
+    return (q[..., 0] | q[..., 1] << 4).to(torch.uint8), s.t().contiguous()
+
+
+def _as_16bit_rows(x, dtype):
+    """x as contiguous (rows, features) in fp16 or bf16 (other types are converted to `dtype`), and its leading sizes."""
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        x = x.to(dtype)
+    return x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
+
+
+class Int4Linear(nn.Module):
+    """Linear layer on 4-bit weights with one fp16 scale per `group_size` inputs; activations stay fp16 or bf16
+    (inference only). Built for few tokens, where its time is that of reading the weight; any number runs."""
+
+    def __init__(self, in_features, out_features, bias=True, group_size=128, dtype=torch.float16):
+        super().__init__()
+        if in_features % 8 != 0:
+            raise ValueError("Int4Linear needs in_features % 8 == 0")
+        if group_size not in (32, 64, 128):
+            raise ValueError("Int4Linear needs group_size 32, 64 or 128")
+        self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
+        self.dtype = dtype
+        self.register_buffer("w_int4", torch.full((out_features, -(-in_features // 128) * 64), 0x88, dtype=torch.uint8))
+        self.register_buffer("w_scale", torch.ones(-(-in_features // group_size), out_features, dtype=torch.float16))
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype))
+        else:
+            self.register_parameter("bias", None)
+
+    def forward(self, x):
+        x2, lead = _as_16bit_rows(x, self.dtype)
+        bias = None if self.bias is None else self.bias.detach().to(x2.dtype)
+        y = _C.int4_linear(x2.detach(), self.w_int4, self.w_scale, bias, self.group_size)
+        return y.reshape(*lead, self.out_features)
+
+    @torch.no_grad()
+    def quantize_weight(self, weight_fp):
+        w, s = quantize_weight_int4(weight_fp.to(self.w_int4.device), self.group_size)
+        self.w_int4.copy_(w)
+        self.w_scale.copy_(s)
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, group_size={self.group_size}")
+
+
+class _GatedLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up):
+        h, g, u = _C.gated_linear(x, w_gate, w_up, b_gate, b_up, save=True)
+        ctx.save_for_backward(x, w_gate, w_up, g, u)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, g, u = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        grads = _C.gated_linear_backward(dh.contiguous(), x, w_gate, w_up, g, u, need[0], need[1] or need[2],
+                                         need[3] or need[4])
+        return tuple(d if n else None for d, n in zip(grads, need))
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None):
+    """SiLU(x w_gate^T + b_gate) * (x w_up^T + b_up), differentiable in every argument. x (..., K), weights (N, K), biases
+    (N), all fp16 or all bf16, K and N multiples of 8. In training the two products are kept in fp32."""
+    x2 = x.reshape(-1, x.shape[-1]).contiguous()
+    w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
+    args = (x2, w_gate, w_up, b_gate, b_up)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        h = _GatedLinearFn.apply(*args)
+    else:
+        h = _C.gated_linear(*args)
+    return h.reshape(*x.shape[:-1], w_gate.shape[0])
+
+
+class GatedLinear(nn.Module):
+    """The gate of a Llama-style MLP, SiLU(gate(x)) * up(x), on fp16 / bf16 weights: one kernel forward, trainable.
+    `forge_b200.quant.quantize(model, scheme="weight_only_int4")` turns it into an `Int4GatedLinear`."""
+
+    def __init__(self, in_features, out_features, bias=False, dtype=torch.float16, device=None):
+        super().__init__()
+        if in_features % 8 != 0 or out_features % 8 != 0:
+            raise ValueError("GatedLinear needs in_features % 8 == 0 and out_features % 8 == 0")
+        self.in_features, self.out_features = in_features, out_features
+        new = lambda *s: nn.Parameter(torch.empty(*s, dtype=dtype, device=device))  # noqa: E731
+        self.w_gate, self.w_up = new(out_features, in_features), new(out_features, in_features)
+        if bias:
+            self.b_gate, self.b_up = new(out_features), new(out_features)
+        else:
+            self.register_parameter("b_gate", None)
+            self.register_parameter("b_up", None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        bound = 1 / math.sqrt(self.in_features)   # as nn.Linear
+        for p in self.parameters():
+            nn.init.uniform_(p, -bound, bound)
+
+    def forward(self, x):
+        return gated_linear(x.to(self.w_gate.dtype), self.w_gate, self.w_up, self.b_gate, self.b_up)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.b_gate is not None}"
+
+
+class Int4GatedLinear(nn.Module):
+    """SiLU(gate(x)) * up(x) on 4-bit weights, one kernel (inference only)."""
+
+    def __init__(self, in_features, out_features, bias=False, group_size=128, dtype=torch.float16):
+        super().__init__()
+        if in_features % 8 != 0:
+            raise ValueError("Int4GatedLinear needs in_features % 8 == 0")
+        if group_size not in (32, 64, 128):
+            raise ValueError("Int4GatedLinear needs group_size 32, 64 or 128")
+        self.in_features, self.out_features, self.group_size = in_features, out_features, group_size
+        self.dtype = dtype
+        for k in ("gate", "up"):
+            self.register_buffer(f"w_{k}_int4",
+                                 torch.full((out_features, -(-in_features // 128) * 64), 0x88, dtype=torch.uint8))
+            self.register_buffer(f"w_{k}_scale",
+                                 torch.ones(-(-in_features // group_size), out_features, dtype=torch.float16))
+            if bias:
+                self.register_parameter(f"b_{k}", nn.Parameter(torch.zeros(out_features, dtype=dtype)))
+            else:
+                self.register_parameter(f"b_{k}", None)
+
+    def forward(self, x):
+        x2, lead = _as_16bit_rows(x, self.dtype)
+        bg, bu = (None if b is None else b.detach().to(x2.dtype) for b in (self.b_gate, self.b_up))
+        h = _C.int4_gated_linear(x2.detach(), self.w_gate_int4, self.w_up_int4, self.w_gate_scale, self.w_up_scale, bg, bu,
+                                 self.group_size)
+        return h.reshape(*lead, self.out_features)
+
+    @torch.no_grad()
+    def quantize_weight(self, w_gate_fp, w_up_fp):
+        for k, w in (("gate", w_gate_fp), ("up", w_up_fp)):
+            q, s = quantize_weight_int4(w.to(self.w_gate_int4.device), self.group_size)
+            getattr(self, f"w_{k}_int4").copy_(q)
+            getattr(self, f"w_{k}_scale").copy_(s)
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.b_gate is not None}, "
+                f"group_size={self.group_size}")

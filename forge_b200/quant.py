@@ -25,9 +25,9 @@ import copy
 import torch
 import torch.nn as nn
 
-from .nn import QuantizedLinear, SparseLinear
+from .nn import GatedLinear, Int4GatedLinear, Int4Linear, QuantizedLinear, SparseLinear
 
-_SCHEMES = ("dynamic_int8", "static_int8", "weight_only_int8")
+_SCHEMES = ("dynamic_int8", "static_int8", "weight_only_int8", "weight_only_int4")
 
 
 def _set_child(model, dotted, new_module):
@@ -68,9 +68,30 @@ def _to_w8a8(linear, sparse):
     return new
 
 
+def _to_int4(m, group_size):
+    """Int4Linear / Int4GatedLinear of a float layer on its device, in its type if that is bf16, else in fp16."""
+    w = m.w_gate if isinstance(m, GatedLinear) else m.weight
+    dtype = torch.bfloat16 if w.dtype == torch.bfloat16 else torch.float16
+    if isinstance(m, GatedLinear):
+        new = Int4GatedLinear(m.in_features, m.out_features, m.b_gate is not None, group_size, dtype).to(w.device)
+        new.quantize_weight(m.w_gate.data, m.w_up.data)
+        if m.b_gate is not None:
+            new.b_gate.data.copy_(m.b_gate.data)
+            new.b_up.data.copy_(m.b_up.data)
+        return new
+    new = Int4Linear(m.in_features, m.out_features, m.bias is not None, group_size, dtype).to(w.device)
+    new.quantize_weight(m.weight.data)
+    if m.bias is not None:
+        new.bias.data.copy_(m.bias.data)
+    return new
+
+
 def quantize(model, calibration_data=None, num_calibration_batches=100, scheme="dynamic_int8", inplace=False,
-             forward_fn=None, *, sparse=False, verbose=True):
-    """Returns `model` with its `nn.Linear` layers replaced by W8A8 layers.
+             forward_fn=None, *, sparse=False, group_size=128, verbose=True):
+    """Returns `model` with its `nn.Linear` layers replaced by W8A8 layers, or with scheme="weight_only_int4" (additive)
+    by layers on 4-bit weights with one scale per `group_size` inputs: `nn.Linear` -> `Int4Linear` (layers with
+    in_features % 8 != 0 become `QuantizedLinear`), `GatedLinear` -> `Int4GatedLinear`. The other schemes leave a
+    `GatedLinear` as it is.
 
     Parameters up to `forward_fn` are the reference's (convert.py:19-26). Additive, keyword only:
     sparse=True prunes each weight 2:4 by magnitude and uses `SparseLinear` where the layer is on a
@@ -79,9 +100,16 @@ def quantize(model, calibration_data=None, num_calibration_batches=100, scheme="
     """
     if scheme not in _SCHEMES:
         raise ValueError(f"unknown scheme {scheme!r}; expected one of {_SCHEMES}")
+    int4 = scheme == "weight_only_int4"
+    if int4 and sparse:
+        raise ValueError("sparse=True is for the INT8 schemes")
     if not inplace:
         model = copy.deepcopy(model)
-    swaps = [(name, _to_w8a8(m, sparse)) for name, m in model.named_modules() if isinstance(m, nn.Linear)]
+    if int4:
+        swaps = [(name, _to_int4(m, group_size) if m.in_features % 8 == 0 else _to_w8a8(m, False))
+                 for name, m in model.named_modules() if isinstance(m, (nn.Linear, GatedLinear))]
+    else:
+        swaps = [(name, _to_w8a8(m, sparse)) for name, m in model.named_modules() if isinstance(m, nn.Linear)]
     for name, new in swaps:
         _set_child(model, name, new)
     if scheme == "static_int8" and calibration_data is not None:
@@ -90,8 +118,9 @@ def quantize(model, calibration_data=None, num_calibration_batches=100, scheme="
         _run_calibration(model, calibration_data, num_calibration_batches, forward_fn, device)
     if verbose:
         n_sparse = sum(isinstance(m, SparseLinear) for _, m in swaps)
-        print(f"forge_b200.quant: converted {len(swaps) - n_sparse} Linear -> QuantizedLinear, "
-              f"{n_sparse} Linear -> SparseLinear")
+        n_int4 = sum(isinstance(m, (Int4Linear, Int4GatedLinear)) for _, m in swaps)
+        print(f"forge_b200.quant: converted {len(swaps) - n_sparse - n_int4} Linear -> QuantizedLinear, "
+              f"{n_sparse} Linear -> SparseLinear" + (f", {n_int4} to 4-bit layers" if int4 else ""))
     return model
 
 

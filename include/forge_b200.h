@@ -201,6 +201,61 @@ int forge_sparse_w8a8_gated_mlp(const void* x, const int8_t* Wg_comp, const uint
                                 const void* bu, const void* bd, void* out, int M, int d_model, int d_ffn,
                                 void* workspace, forge_stream_t stream);
 
+/* ---------------------------------------------------------------- gated linear layer, 16-bit weights (additive) */
+
+/* Element types of the entry points that take more than fp16. */
+enum {
+    FORGE_DTYPE_F32 = 0,
+    FORGE_DTYPE_F16 = 1,
+    FORGE_DTYPE_BF16 = 2
+};
+
+/* No counterpart in the reference. The gate of a Llama-style MLP on unquantized weights, forward and backward - the layer
+ * that forge_int8_gated_gemm and forge_int4_gated_linear serve after quantization:
+ *   g = x Wg^T + bg,  u = x Wu^T + bu,  h = SiLU(g) * u
+ * x (M,K), Wg / Wu (N,K), bg / bu (N, may be NULL), h (M,N), all of `dtype` (FORGE_DTYPE_F16 or _BF16). g_out / u_out:
+ * (M,N) fp32 that receive g and u for the backward pass, both or neither NULL. Products, gate and sums are evaluated in
+ * fp32, h is rounded once. Needs K % 8 == 0, N % 8 == 0 and 16-byte aligned matrices (FORGE_B200_BAD_SHAPE otherwise). */
+int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void* bg, const void* bu, void* h,
+                       float* g_out, float* u_out, int M, int K, int N, int dtype, forge_stream_t stream);
+
+/* Its gradients for dh (M,N): dx (M,K), dWg / dWu (N,K, both or neither NULL), dbg / dbu (N), each NULL when not wanted,
+ * all of `dtype`; g and u as the forward call wrote them. The gradients of g and u are rounded to `dtype` before the
+ * products, everything else is fp32; the order of every sum is fixed. `workspace` is caller-owned device memory of
+ * forge_gated_linear_backward_workspace_bytes(M, N) bytes, 256-byte aligned. With M <= 0 nothing is written, the
+ * gradients of the weights included (they are zero). */
+unsigned long long forge_gated_linear_backward_workspace_bytes(int M, int N);
+int forge_gated_linear_backward(const void* dh, const void* x, const void* Wg, const void* Wu, const float* g,
+                                const float* u, void* dx, void* dWg, void* dWu, void* dbg, void* dbu, int M, int K,
+                                int N, int dtype, void* workspace, forge_stream_t stream);
+
+/* ---------------------------------------------------------------- 4-bit weights with group scales (additive) */
+
+/* No counterpart in the reference. A weight row's inputs are cut into groups of group_size (32, 64 or 128, the last one
+ * may be short); w[n,k] = w_scale[k / group_size, n] * q[n,k], q an integer in -8..7.
+ *
+ * w_int4: (N, ceil(K/128) * 64) bytes. Eight neighbouring weights make one little-endian 32-bit word: weight 2i in nibble
+ * i (bits 4i..4i+3), weight 2i+1 in nibble i+4, each stored as q + 8. Of the 16 words of a block of 128 inputs, word
+ * 4t+j holds the block's run 4j+t of eight (t, j in 0..3). Inputs past K are stored as q = 0.
+ * w_scale: (ceil(K/group_size), N) fp16.
+ *
+ * forge_prepare_weight_int4: weight (N,K) of `dtype` (FORGE_DTYPE_*) -> both, with scale = fp16(absmax / 7) and
+ * q = clamp(round_half_even(w / scale), -7, 7). A group that holds an infinity or a NaN, or whose scale is beyond
+ * fp16, gets a NaN scale. Needs K % 8 == 0 and 16-byte aligned weight and w_int4 (FORGE_B200_BAD_SHAPE otherwise). */
+int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, void* w_scale, int N, int K,
+                              int group_size, forge_stream_t stream);
+
+/* output (M,N) = x (M,K) W^T + bias (N, may be NULL); x, bias and output of `dtype` (FORGE_DTYPE_F16 or _BF16). Sums in
+ * fp32, one rounding at the end. Needs K % 8 == 0, 16-byte aligned x and w_int4 (FORGE_B200_BAD_SHAPE otherwise). */
+int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale, const void* bias, void* output, int M,
+                      int K, int N, int group_size, int dtype, forge_stream_t stream);
+
+/* output (M,N) = SiLU(x Wg^T + bg) * (x Wu^T + bu) with both weights in that form, in one kernel: the gate of a 4-bit
+ * MLP. Arguments and preconditions as above. */
+int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t* wu_int4, const void* wg_scale,
+                            const void* wu_scale, const void* bg, const void* bu, void* output, int M, int K, int N,
+                            int group_size, int dtype, forge_stream_t stream);
+
 /* ---------------------------------------------------------------- forge::sparsity */
 
 /* forge::sparsity::prune_compress_24 - include/forge/sparsity/prune_compress.cuh:23-30,
@@ -264,7 +319,8 @@ int forge_int8_conv_transpose2d_k2s2_forward(const void* input, const int8_t* we
  * the last reset, FORGE_B200_DEVICE_TIMEOUT when one has (FORGE_B200_LAUNCH_FAILED when the word
  * cannot be read). forge_b200_device_status_raw returns the recorded code itself:
  *   100-104 dense GEMM, 200-204 2:4-sparse GEMM, 300-304 / 400-404 their CTA-pair forms,
- *   500-506 fused quantize + sparse GEMM, 600-605 convolution; within a range x00 = misaligned
+ *   500-506 fused quantize + sparse GEMM, 600-605 convolution, 700-704 gated linear layer on 16-bit
+ *   weights; within a range x00 = misaligned
  *   shared memory, x01 = producer waiting for a free stage, x02 = MMA issuer waiting for a drained
  *   accumulator, x03 = MMA issuer waiting for operands, x04 and up = epilogue / gather waits.
  * Both synchronise the device; reset != 0 clears the word after reading it. */

@@ -1,0 +1,308 @@
+"""4-bit weights with group scales on the GPU: preparation bit for bit, the linear and the gated layer against 64-bit
+products, at the sizes, groups and values where they can go wrong, and the calls they refuse."""
+import pytest
+import torch
+
+import float_ref as R
+from forge_b200 import _forge_C as C
+from forge_b200 import _lib
+from forge_b200.nn import Int4GatedLinear, Int4Linear, quantize_weight_int4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _ok():
+    torch.cuda.synchronize()
+    assert C.device_status() == 0
+
+
+def _weight(N, K, group, gen, scale=0.05):
+    """Packed weight with every nibble value, prepared on the CPU."""
+    w, s = quantize_weight_int4(torch.randn(N, K, generator=gen) * scale, group)
+    w = torch.where(torch.rand(w.shape, generator=gen) < 0.1, torch.randint(0, 256, w.shape, generator=gen).to(torch.uint8), w)
+    tail = K % 128   # inputs past K are stored as zeros
+    if tail:
+        blk = w[:, -64:].view(N, 4, 4, 4)
+        run = 4 * torch.arange(4)[None, :] + torch.arange(4)[:, None]   # [t][j]
+        blk[:, run * 8 >= tail] = 0x88
+    return w.to(DEV), s.to(DEV)
+
+
+# ------------------------------------------------------------------------------------------------ preparation
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("N,K", [(1, 8), (3, 120), (17, 128), (40, 136), (130, 1000), (5, 4096)])
+def test_prepare_equals_the_cpu_recipe(N, K, group, dtype):
+    g = torch.Generator().manual_seed(N * 7 + K + group)
+    w = (torch.randn(N, K, generator=g) * torch.rand(N, 1, generator=g)).to(dtype)
+    w[0, :min(K, 40)] = 0
+    want = quantize_weight_int4(w, group)
+    got = C.prepare_weight_int4(w.to(DEV), group)
+    _ok()
+    assert torch.equal(got[0].cpu(), want[0])
+    assert torch.equal(got[1].cpu().view(torch.int16), want[1].view(torch.int16))
+
+
+def test_prepare_on_rounding_borders():
+    """Weights exactly on and one step beside every border n + 1/2 of every scale."""
+    rows = []
+    for i, s in enumerate([0.0078125, 0.00731, 0.9, 1.7e-5, 3.0]):
+        s = torch.tensor(s).half().float()
+        n = torch.arange(-7, 7).float() + 0.5
+        w = torch.cat([n * s, torch.nextafter(n * s, torch.tensor(9.0)), torch.nextafter(n * s, torch.tensor(-9.0))])
+        row = torch.zeros(128)
+        row[: len(w)] = w
+        row[-1] = 7 * s
+        rows.append(row)
+    w = torch.stack(rows)
+    want, got = quantize_weight_int4(w, 128), C.prepare_weight_int4(w.to(DEV), 128)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+def test_prepare_of_unusual_values():
+    w = torch.zeros(6, 64)
+    w[0, 3] = float("inf")
+    w[1, 40] = float("nan")
+    w[2, 0] = 7 * 65504.0
+    w[3, 0] = 3e38
+    w[4, 0] = 1e-12                 # the scale rounds to zero: all weights are zero
+    w[5] = torch.linspace(-1e-6, 1e-6, 64)   # a subnormal scale
+    want, got = quantize_weight_int4(w, 32), C.prepare_weight_int4(w.to(DEV), 32)
+    assert torch.equal(got[0].cpu(), want[0])
+    assert torch.equal(got[1].cpu().isnan(), want[1].isnan()) and torch.equal(got[1].cpu().nan_to_num(), want[1].nan_to_num())
+    nan = got[1].cpu().isnan()
+    assert nan[0, 0] and not nan[1, 0] and nan[1, 1] and not nan[0, 1] and not nan[0, 2] and nan[0, 3]
+
+
+def test_prepare_of_views():
+    big = torch.randn(300, 264, device=DEV)
+    want = C.prepare_weight_int4(big[10:40, 8:200].clone(), 64)
+    got = C.prepare_weight_int4(big[10:40, 8:200], 64)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    odd = torch.randn(30 * 64 + 1, device=DEV)[1:].view(30, 64)   # contiguous, not 16-byte aligned
+    want, got = C.prepare_weight_int4(odd.clone(), 64), C.prepare_weight_int4(odd, 64)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------------------------------------ linear, gated
+
+SHAPES = [(1, 8, 1), (1, 64, 17), (1, 4096, 100), (2, 120, 16), (5, 2056, 33), (7, 520, 272), (8, 1000, 15), (9, 136, 48),
+          (16, 256, 31), (17, 384, 130), (33, 520, 64), (64, 1024, 256), (100, 72, 257), (129, 648, 300), (300, 2048, 520)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_int4_linear(M, K, N, group, dtype):
+    g = torch.Generator().manual_seed(M + 3 * K + 5 * N + group)
+    x = (torch.randn(M, K, generator=g) * (1 + 9 * (torch.rand(K, generator=g) < 0.05))).to(TYPES[dtype]).to(DEV)
+    w, s = _weight(N, K, group, g)
+    bias = torch.randn(N, generator=g).to(TYPES[dtype]).to(DEV) if (M + N) % 2 else None
+    y = C.int4_linear(x, w, s, bias, group)
+    _ok()
+    want, err = linear_bound(x, R.unpack_int4(w, s, K, group), bias)
+    R.close_rounded(y, want, err)
+
+
+def linear_bound(x, w, b):
+    """Above `MANY` tokens a weight is rounded once to the activations' type before the products."""
+    y, err = R.linear(x, w, b)
+    if x.shape[0] > MANY:
+        err = err + x.double().abs() @ R.half_step(w, x.dtype).t()
+    return y, err
+
+
+MANY = 10 ** 9
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_int4_gated_linear(M, K, N, group, dtype):
+    g = torch.Generator().manual_seed(2 * M + 3 * K + 5 * N + group)
+    x = torch.randn(M, K, generator=g).to(TYPES[dtype]).to(DEV)
+    (wg, sg), (wu, su) = _weight(N, K, group, g), _weight(N, K, group, g)
+    bg, bu = ((torch.randn(N, generator=g) * 0.3).to(TYPES[dtype]).to(DEV) if (M + N) % 2 else None for _ in range(2))
+    h = C.int4_gated_linear(x, wg, wu, sg, su, bg, bu, group)
+    _ok()
+    (gv, eg), (uv, eu) = (linear_bound(x, R.unpack_int4(w, s, K, group), b) for w, s, b in ((wg, sg, bg), (wu, su, bu)))
+    silu = gv * torch.sigmoid(gv)
+    err = 1.1 * eg * (uv.abs() + eu) + silu.abs() * eu + R._fn_rel(gv) * (silu * uv).abs() + 2.0 ** -120
+    R.close_rounded(h, silu * uv, err)
+
+
+@pytest.mark.parametrize("M", [1, 8, 40])
+def test_repeated_calls_give_the_same_bits(M):
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, 4096, generator=g).half().to(DEV)
+    w, s = _weight(200, 4096, 64, g)
+    y = C.int4_linear(x, w, s, None, 64)
+    for _ in range(5):
+        assert torch.equal(C.int4_linear(x, w, s, None, 64), y)
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_infinities_and_nans_stay_where_they_belong(M):
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(M, 264, generator=g).half().to(DEV)
+    w, s = _weight(50, 264, 32, g)
+    y = C.int4_linear(x, w, s, None, 32)
+    xn, sn = x.clone(), s.clone()
+    xn[1, 263] = float("nan")
+    xn[2, 0] = float("inf")
+    sn[8, 7] = float("nan")
+    z = C.int4_linear(xn, w, sn, None, 32)
+    assert z[1].isnan().all() and not z[2].isfinite().any() and z[:, 7].isnan().all()
+    keep = torch.ones_like(y, dtype=torch.bool)
+    keep[1:3] = False
+    keep[:, 7] = False
+    assert torch.equal(z[keep], y[keep])
+
+
+def test_large_results_overflow_only_at_the_end():
+    """Products beyond fp16 that cancel: sums are fp32."""
+    x = torch.full((2, 64), 300.0, device=DEV).half()
+    x[1, 32:] = -300.0
+    q = torch.full((4, 64), 7.0) * 60
+    w, s = quantize_weight_int4(q, 32)
+    y = C.int4_linear(x, w.to(DEV), s.to(DEV), None, 32)
+    assert y[0].isinf().all() and (y[1] == 0).all()
+
+
+def test_no_tokens_no_outputs():
+    w, s = C.prepare_weight_int4(torch.randn(24, 64, device=DEV), 64)
+    assert C.int4_linear(torch.empty(0, 64, device=DEV).half(), w, s, None, 64).shape == (0, 24)
+    x = torch.randn(3, 64, device=DEV).half()
+    assert C.int4_linear(x, w[:0], s[:, :0].contiguous(), None, 64).shape == (3, 0)
+    assert C.int4_gated_linear(x[:0], w, w, s, s, None, None, 64).shape == (0, 24)
+
+
+def test_weight_past_32_bit_offsets():
+    """A weight of more than 2^31 bytes: its last rows are read where they are."""
+    K, N = 65536, 70000
+    g = torch.Generator().manual_seed(0)
+    w = torch.full((N, K // 2), 0x88, dtype=torch.uint8, device=DEV)
+    s = torch.ones(K // 128, N, dtype=torch.float16, device=DEV)
+    tail, st = _weight(16, K, 128, g)
+    w[-16:], s[:, -16:] = tail, st
+    for M in (1, 40):
+        x = torch.randn(M, K, generator=g).half().to(DEV)
+        y = C.int4_linear(x, w, s)
+        _ok()
+        R.close_rounded(y[:, -16:], *linear_bound(x, R.unpack_int4(tail, st, K, 128), None))
+        assert (y[:, :-16] == 0).all()
+
+
+def test_on_another_stream_and_in_a_graph():
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(4, 512, generator=g).half().to(DEV)
+    big = torch.randn(80, 512, generator=g).half().to(DEV)
+    w, s = _weight(300, 512, 64, g)
+    want, want_big = C.int4_linear(x, w, s, None, 64), C.int4_gated_linear(big, w, w, s, s, None, None, 64)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = C.int4_linear(x, w, s, None, 64)
+        got_big = C.int4_gated_linear(big, w, w, s, s, None, None, 64)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got_big, want_big)
+    graph = torch.cuda.CUDAGraph()
+    xin = torch.zeros_like(x)
+    bin_ = torch.zeros_like(big)
+    with torch.cuda.graph(graph):
+        y = C.int4_linear(xin, w, s, None, 64)
+        z = C.int4_gated_linear(bin_, w, w, s, s, None, None, 64)
+    for scale in (1, 2):
+        xin.copy_(x * scale)
+        bin_.copy_(big * scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, C.int4_linear(x * scale, w, s, None, 64))
+        assert torch.equal(z, C.int4_gated_linear(big * scale, w, w, s, s, None, None, 64))
+
+
+def test_rows_behind_the_output_stay():
+    """Through the C ABI, into the middle of a larger buffer."""
+    g = torch.Generator().manual_seed(3)
+    w, s = _weight(37, 256, 128, g)
+    for M in (3, 50):
+        x = torch.randn(M, 256, generator=g).half().to(DEV)
+        out = torch.full((M + 2, 37), 7.0, device=DEV).half()
+        _lib.call("forge_int4_linear", x.data_ptr(), w.data_ptr(), s.data_ptr(), 0, out[1:].data_ptr(), M, 256, 37, 128, 1,
+                  torch.cuda.current_stream().cuda_stream)
+        assert (out[0] == 7).all() and (out[-1] == 7).all()
+        assert torch.equal(out[1:-1], C.int4_linear(x, w, s))
+
+
+def test_an_unaligned_activation_is_taken():
+    g = torch.Generator().manual_seed(5)
+    w, s = _weight(40, 128, 32, g)
+    buf = torch.randn(4 * 128 + 3, generator=g).half().to(DEV)
+    x = buf[3:].view(4, 128)
+    assert torch.equal(C.int4_linear(x, w, s, None, 32), C.int4_linear(x.clone(), w, s, None, 32))
+
+
+def test_refusals():
+    x = torch.randn(4, 128, device=DEV).half()
+    w, s = C.prepare_weight_int4(torch.randn(32, 128, device=DEV), 64)
+    call = lambda x=x, w=w, s=s, b=None, g=64: C.int4_linear(x, w, s, b, g)  # noqa: E731
+    call()
+    with pytest.raises(TypeError):
+        call(x=x.float())
+    with pytest.raises(TypeError):
+        call(s=s.float())
+    with pytest.raises(TypeError):
+        call(b=torch.zeros(32, device=DEV))
+    with pytest.raises(ValueError):
+        call(x=x[:, :124].contiguous())            # not a multiple of 8
+    with pytest.raises(ValueError):
+        call(x=x[:, :0])
+    with pytest.raises(ValueError):
+        call(x=x[0])
+    with pytest.raises(ValueError):
+        call(x=x.t().contiguous().t())             # strided
+    with pytest.raises(ValueError):
+        call(g=96)
+    with pytest.raises(ValueError):
+        call(g=128)                                # the scales are of another group size
+    with pytest.raises(ValueError):
+        call(w=w[:, :32].contiguous())
+    with pytest.raises(ValueError):
+        call(b=torch.zeros(31, device=DEV).half())
+    with pytest.raises(ValueError):
+        call(x=x.cpu())
+    with pytest.raises(ValueError):
+        C.int4_gated_linear(x, w, w[:16], s, s[:, :16].contiguous(), None, None, 64)
+    with pytest.raises(ValueError):
+        C.prepare_weight_int4(torch.randn(32, 100, device=DEV), 64)
+    with pytest.raises(ValueError):
+        C.prepare_weight_int4(torch.randn(32, 128, device=DEV), 16)
+    _ok()
+
+
+# ------------------------------------------------------------------------------------------------ modules
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_modules(dtype):
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(2, 3, 264, generator=g).to(TYPES[dtype]).to(DEV)
+    w, w2 = torch.randn(2, 48, 264, generator=g).mul(0.05).to(DEV)
+    m = Int4Linear(264, 48, group_size=32, dtype=TYPES[dtype]).to(DEV)
+    m.quantize_weight(w)
+    m.bias.data.normal_()
+    y = m(x)
+    assert y.shape == (2, 3, 48) and y.dtype == x.dtype
+    want, err = R.linear(x.view(6, 264), R.unpack_int4(m.w_int4, m.w_scale, 264, 32), m.bias)
+    R.close_rounded(y.view(6, 48), want, err)
+    gm = Int4GatedLinear(264, 48, group_size=32, dtype=TYPES[dtype]).to(DEV)
+    gm.quantize_weight(w, w2)
+    h = gm(x.transpose(0, 1))
+    want, err, _ = R.gate(x.transpose(0, 1).reshape(6, 264), R.unpack_int4(gm.w_gate_int4, gm.w_gate_scale, 264, 32),
+                          R.unpack_int4(gm.w_up_int4, gm.w_up_scale, 264, 32), None, None)
+    R.close_rounded(h.reshape(6, 48), want, err)
+    other = Int4Linear(264, 48, group_size=32, dtype=TYPES[dtype]).to(DEV)
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other(x), y)

@@ -17,7 +17,8 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    # the handle itself: building a torch.cuda.Stream object first takes 3 us
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _on(t):
@@ -253,11 +254,20 @@ def prepare_weight_int4(weight, group_size=128):
 def _int4_operand(x, name, w, s, b, N, group_size):
     """Checks one 4-bit weight with its scales and bias against x (M, K) and N outputs."""
     K = x.size(1)
-    _chk(x, **{name + "_int4": (w, _u8), name + "_scale": (s, _f16), "bias of " + name: (b, x.dtype)})
-    _shape(**{name + "_int4": (w, (N, (K + 127) // 128 * _BYTES_PER_BLOCK)),
-              name + "_scale": (s, ((K + group_size - 1) // group_size, N)), "bias of " + name: (b, (N,))})
-    if w.data_ptr() % 16 != 0:
-        raise ValueError(f"{name}_int4: must start at a 16-byte aligned address")
+    dev = x.device
+    if w.dtype != _u8 or s.dtype != _f16 or (b is not None and b.dtype != x.dtype):
+        raise TypeError(f"{name}_int4, {name}_scale, bias: expected {_u8}, {_f16}, {x.dtype}, "
+                        f"got {w.dtype}, {s.dtype}, {None if b is None else b.dtype}")
+    if w.shape != (N, (K + 127) // 128 * _BYTES_PER_BLOCK) or s.shape != ((K + group_size - 1) // group_size, N) or (
+            b is not None and b.shape != (N,)):
+        raise ValueError(f"{name}_int4 {tuple(w.shape)}, {name}_scale {tuple(s.shape)}, bias "
+                         f"{None if b is None else tuple(b.shape)} do not fit {K} inputs in groups of {group_size}, {N} outputs")
+    if w.device != dev or s.device != dev or (b is not None and b.device != dev):
+        raise ValueError(f"{name}_int4, {name}_scale and bias must be on {dev}")
+    if not (w.is_contiguous() and s.is_contiguous() and (b is None or b.is_contiguous())):
+        raise ValueError(f"{name}_int4, {name}_scale and bias must be contiguous")
+    if w.data_ptr() % 16 != 0 or s.data_ptr() % 4 != 0:
+        raise ValueError(f"{name}_int4 must start at a 16-byte aligned address, {name}_scale at a 4-byte aligned one")
 
 
 def int4_linear(x, w_int4, w_scale, bias=None, group_size=128):
@@ -269,7 +279,7 @@ def int4_linear(x, w_int4, w_scale, bias=None, group_size=128):
     N = w_int4.size(0)
     _int4_operand(x, "w", w_int4, w_scale, bias, N, group_size)
     x = _aligned(x)
-    output = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    output = x.new_empty((M, N))
     with _on(x):
         _lib.call("forge_int4_linear", _ptr(x), _ptr(w_int4), _ptr(w_scale), _ptr(bias), _ptr(output), M, K, N,
                   group_size, dtype, _stream())
@@ -286,7 +296,7 @@ def int4_gated_linear(x, wg_int4, wu_int4, wg_scale, wu_scale, bg=None, bu=None,
     _int4_operand(x, "wg", wg_int4, wg_scale, bg, N, group_size)
     _int4_operand(x, "wu", wu_int4, wu_scale, bu, N, group_size)
     x = _aligned(x)
-    output = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    output = x.new_empty((M, N))
     with _on(x):
         _lib.call("forge_int4_gated_linear", _ptr(x), _ptr(wg_int4), _ptr(wu_int4), _ptr(wg_scale), _ptr(wu_scale),
                   _ptr(bg), _ptr(bu), _ptr(output), M, K, N, group_size, dtype, _stream())

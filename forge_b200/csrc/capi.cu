@@ -10,7 +10,6 @@
 #include "gemm_fq.cuh"
 #include "int4.cuh"
 #include "kernels.cuh"
-#include "wstream.cuh"
 
 using namespace fb200;
 
@@ -55,6 +54,7 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, const __half*
 }
 
 inline bool is_16bit(int dtype) { return dtype == FORGE_DTYPE_F16 || dtype == FORGE_DTYPE_BF16; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline bool is_group(int g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
@@ -349,10 +349,12 @@ int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale,
                       int K, int N, int group_size, int dtype, forge_stream_t stream) {
     if (M <= 0 || K <= 0 || N <= 0) return kOk;
     if (x == nullptr || w_int4 == nullptr || w_scale == nullptr || output == nullptr) return kBadPointer;
-    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(w_int4)) return kBadShape;
+    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(w_int4) ||
+        !aligned4(w_scale))
+        return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return wstream(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
-                   dtype == FORGE_DTYPE_BF16, S(stream));
+    return int4_stream(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
+                       dtype == FORGE_DTYPE_BF16, S(stream));
 }
 
 int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t* wu_int4, const void* wg_scale,
@@ -363,11 +365,11 @@ int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t
         output == nullptr)
         return kBadPointer;
     if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(wg_int4) ||
-        !aligned16(wu_int4))
+        !aligned16(wu_int4) || !aligned4(wg_scale) || !aligned4(wu_scale))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return wstream(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
-                   dtype == FORGE_DTYPE_BF16, S(stream));
+    return int4_stream(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
+                       dtype == FORGE_DTYPE_BF16, S(stream));
 }
 
 int forge_prune_compress_24(const int8_t* weight, int8_t* compressed, uint8_t* metadata_raw, int N, int K,

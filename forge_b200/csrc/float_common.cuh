@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -31,34 +32,29 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Word of 8 four-bit weights (weight 2i in nibble i, weight 2i + 1 in nibble i + 4, stored as the integer + 8) ->
-// four pairs of 16-bit floats. A nibble placed in the low mantissa bits of 1024 (fp16) or 128 (bf16) is that number
-// plus the nibble, exactly; subtracting the offset + 8 leaves the integer, exactly.
+// (v & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
+    return r;
+}
+
+// D = A B + C, A 16 rows x 16 inputs, B 16 inputs x 8 tokens; C is D, or zero (`first`, a constant where it is inlined)
+#define FB200_MMA(TYPE)                                                                                                 \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                                 \
+                 ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"                                       \
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                       \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(first ? 0.f : d[0]), "f"(first ? 0.f : d[1]), \
+                   "f"(first ? 0.f : d[2]), "f"(first ? 0.f : d[3]))
 template <typename T>
-struct Int4Pairs;
-template <>
-struct Int4Pairs<__half> {
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&f)[4]) {
-        const __half2 off = __half2half2(__ushort_as_half(0x6408));   // 1032
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t b = ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
-            const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-            f[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
+__device__ __forceinline__ void mma16816(bool first, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) {
+        FB200_MMA("f16");
+    } else {
+        FB200_MMA("bf16");
     }
-};
-template <>
-struct Int4Pairs<__nv_bfloat16> {
-    static __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&f)[4]) {
-        const __nv_bfloat162 off = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));   // 136
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t b = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), off);
-            f[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-    }
-};
+}
+#undef FB200_MMA
 
 }  // namespace fb200

@@ -26,7 +26,6 @@
 #include "gated_linear.cuh"
 #include "gemm_dense.cuh"
 #include "ptx.cuh"
-#include "wstream.cuh"
 
 namespace fb200 {
 
@@ -529,7 +528,7 @@ int gate_backward(const void* dh, const float* g, const float* u, void* dg, void
 int gated_linear(const void* x, const void* wg, const void* wu, const void* bg, const void* bu, void* h, float* g,
                  float* u, int M, int K, int N, bool bf16, cudaStream_t stream) {
     // a few tokens: one pass over the weights without tensor-memory tiles that would be mostly empty
-    if (g == nullptr && M <= 16) return wstream(x, wg, wu, nullptr, nullptr, bg, bu, h, M, K, N, 0, bf16, stream);
+    if (g == nullptr && M <= 16) return gated_stream(x, wg, wu, bg, bu, h, M, K, N, bf16, stream);
     Maps m = {};
     const CUtensorMapDataType t = type16(bf16), f = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     if (!encode(&m.a[0], t, 2, x, K, M, 128) || !encode(&m.b[0], t, 2, wg, K, N, 128) ||

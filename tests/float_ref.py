@@ -25,11 +25,23 @@ def unpack_int4(w_int4, w_scale, K, group):
     return (q - 8).double() * w_scale.double().t()[:, k // group].reshape(N, K)
 
 
-def linear(x, w, b):
-    """y and a bound on the fp32 evaluation's error, before any rounding of y."""
+def int4_sizes(w_scale, K, group, dtype):
+    """What `linear` takes as the sizes of 4-bit weights: few tokens are multiplied with q + 8 (bf16: q + 24), from which
+    as much is taken off again, so a product's parts are as large as (|q| + 16) s (bf16: 48), |q| <= 8."""
+    s = w_scale.double().abs().t()[:, torch.arange(K, device=w_scale.device) // group]
+    return s.reshape(w_scale.shape[1], K) * (24 if dtype == torch.float16 else 56)
+
+
+def linear(x, w, b, sizes=None, chain=None):
+    """y and a bound on the fp32 evaluation's error, before any rounding of y. `sizes`: of the products' parts, where they
+    are larger than |w|; `chain`: inputs that are summed at a time, where that is not all of them (then the sums of the
+    K / chain pieces are added in fp32, each addition off by half a step of at most the sum of sizes)."""
     x, w = x.double(), w.double()
     y = x @ w.t()
-    err = (x.shape[1] + 64) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+    K = x.shape[1]
+    err = ((chain or K) + 64) * 2.0 ** -23 * (x.abs() @ (w if sizes is None else sizes).abs().t())
+    if chain:
+        err = err + (K / chain + 64) * 2.0 ** -24 * (x.abs() @ w.abs().t())
     if b is not None:
         y = y + b.double()
         err = err + 2.0 ** -24 * y.abs()
@@ -42,14 +54,17 @@ def _fn_rel(g):
     return (2 + 1.173 * g.abs() + 5) * 2.0 ** -23
 
 
-def gate(x, wg, wu, bg, bu):
-    g, eg = linear(x, wg, bg)
-    u, eu = linear(x, wu, bu)
-    s = torch.sigmoid(g)
-    h = g * s * u
+def gate_of(gate, up):
+    """SiLU(g) u and its bound from (g, bound) and (u, bound)."""
+    (g, eg), (u, eu) = gate, up
+    silu = g * torch.sigmoid(g)
     # |SiLU'| <= 1.1
-    err = 1.1 * eg * (u.abs() + eu) + (g * s).abs() * eu + _fn_rel(g) * h.abs() + 2.0 ** -120
-    return h, err, (g, eg, u, eu)
+    return silu * u, 1.1 * eg * (u.abs() + eu) + silu.abs() * eu + _fn_rel(g) * (silu * u).abs() + 2.0 ** -120
+
+
+def gate(x, wg, wu, bg, bu):
+    g, u = linear(x, wg, bg), linear(x, wu, bu)
+    return (*gate_of(g, u), (*g, *u))
 
 
 def gate_backward(dh, x, wg, wu, saved, dtype):

@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 SHAPES = [(1, 8, 8), (1, 512, 264), (2, 72, 16), (8, 264, 200), (9, 1000, 48), (16, 64, 136), (17, 64, 64), (33, 200, 128),
-          (128, 256, 256), (130, 328, 264), (257, 512, 520), (300, 1032, 136), (513, 136, 1032), (700, 640, 1288)]
+          (128, 256, 256), (130, 328, 264), (257, 512, 520), (300, 1032, 136), (513, 136, 1032), (700, 640, 1288), (3, 4104, 20008), (12, 1160, 9480)]
 
 
 def _ok():
@@ -294,9 +294,11 @@ def test_a_block_is_trained_then_served_with_4_bit_weights(dtype):
     one = x[0, :1]
     g4, d4 = served.gate_up, served.down
     h = g4(one)
-    want, err, _ = R.gate(one, R.unpack_int4(g4.w_gate_int4, g4.w_gate_scale, 128, 32),
-                          R.unpack_int4(g4.w_up_int4, g4.w_up_scale, 128, 32), block.gate_up.b_gate, block.gate_up.b_up)
-    R.close_rounded(h, want, err)
-    y, err = R.linear(h, R.unpack_int4(d4.w_int4, d4.w_scale, 264, 32), d4.bias)
-    R.close_rounded(d4(h), y, err)
+
+    def product(v, w, sc, b):
+        K = v.shape[1]
+        return R.linear(v, R.unpack_int4(w, sc, K, 32), b, R.int4_sizes(sc, K, 32, t), 32)
+    R.close_rounded(h, *R.gate_of(product(one, g4.w_gate_int4, g4.w_gate_scale, block.gate_up.b_gate),
+                                  product(one, g4.w_up_int4, g4.w_up_scale, block.gate_up.b_up)))
+    R.close_rounded(d4(h), *product(h, d4.w_int4, d4.w_scale, d4.bias))
     assert torch.equal(served(one), one + d4(h))

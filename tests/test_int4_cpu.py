@@ -117,12 +117,14 @@ def test_c_refusals():
         return lib.forge_int4_linear(x, w, s, 0, o, M, K, N, group, dtype, 0)
     assert [lin(M=0), lin(K=0), lin(N=-3)] == [0, 0, 0]
     assert [lin(x=0), lin(w=0), lin(s=0), lin(o=0)] == [BAD_POINTER] * 4
-    assert [lin(K=60), lin(group=16), lin(group=0), lin(dtype=0), lin(dtype=3), lin(x=odd), lin(w=odd)] == [BAD_SHAPE] * 7
+    assert [lin(K=60), lin(group=16), lin(group=0), lin(dtype=0), lin(dtype=3), lin(x=odd), lin(w=odd),
+            lin(s=p + 2)] == [BAD_SHAPE] * 8
 
     def gated(x=p, g=p, u=p, sg=p, su=p, o=p, M=4, K=64, N=16, group=64, dtype=2):
         return lib.forge_int4_gated_linear(x, g, u, sg, su, 0, 0, o, M, K, N, group, dtype, 0)
     assert [gated(M=0), gated(x=0), gated(g=0), gated(u=0), gated(sg=0), gated(su=0), gated(o=0)] == [0] + [BAD_POINTER] * 6
-    assert [gated(K=4), gated(group=8), gated(dtype=0), gated(x=odd), gated(g=odd), gated(u=odd)] == [BAD_SHAPE] * 6
+    assert [gated(K=4), gated(group=8), gated(dtype=0), gated(x=odd), gated(g=odd), gated(u=odd),
+            gated(sg=p + 2), gated(su=p + 2)] == [BAD_SHAPE] * 8
 
     def prep(w=p, dtype=0, o=p, s=p, N=4, K=64, group=64):
         return lib.forge_prepare_weight_int4(w, dtype, o, s, N, K, group, 0)

@@ -103,19 +103,12 @@ def test_int4_linear(M, K, N, group, dtype):
     bias = torch.randn(N, generator=g).to(TYPES[dtype]).to(DEV) if (M + N) % 2 else None
     y = C.int4_linear(x, w, s, bias, group)
     _ok()
-    want, err = linear_bound(x, R.unpack_int4(w, s, K, group), bias)
-    R.close_rounded(y, want, err)
+    R.close_rounded(y, *linear_bound(x, w, s, bias, group))
 
 
-def linear_bound(x, w, b):
-    """Above `MANY` tokens a weight is rounded once to the activations' type before the products."""
-    y, err = R.linear(x, w, b)
-    if x.shape[0] > MANY:
-        err = err + x.double().abs() @ R.half_step(w, x.dtype).t()
-    return y, err
-
-
-MANY = 10 ** 9
+def linear_bound(x, w, s, b, group):
+    K = x.shape[1]
+    return R.linear(x, R.unpack_int4(w, s, K, group), b, R.int4_sizes(s, K, group, x.dtype), group)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -128,10 +121,23 @@ def test_int4_gated_linear(M, K, N, group, dtype):
     bg, bu = ((torch.randn(N, generator=g) * 0.3).to(TYPES[dtype]).to(DEV) if (M + N) % 2 else None for _ in range(2))
     h = C.int4_gated_linear(x, wg, wu, sg, su, bg, bu, group)
     _ok()
-    (gv, eg), (uv, eu) = (linear_bound(x, R.unpack_int4(w, s, K, group), b) for w, s, b in ((wg, sg, bg), (wu, su, bu)))
-    silu = gv * torch.sigmoid(gv)
-    err = 1.1 * eg * (uv.abs() + eu) + silu.abs() * eu + R._fn_rel(gv) * (silu * uv).abs() + 2.0 ** -120
-    R.close_rounded(h, silu * uv, err)
+    R.close_rounded(h, *R.gate_of(linear_bound(x, wg, sg, bg, group), linear_bound(x, wu, su, bu, group)))
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("M,K,N", [(1, 16384, 20000), (9, 8200, 13001), (40, 4104, 30001)])
+def test_several_passes_over_the_rows(M, K, N, group):
+    """More rows than the SMs hold at a time, more columns than a ring."""
+    g = torch.Generator().manual_seed(K)
+    x = torch.randn(M, K, generator=g).half().to(DEV)
+    w = torch.randint(0, 256, (N, -(-K // 128) * 64), generator=g).to(torch.uint8).to(DEV)
+    s = (torch.rand(-(-K // group), N, generator=g) * 0.01 + 0.001).half().to(DEV)
+    y = C.int4_linear(x, w, s, None, group)
+    _ok()
+    R.close_rounded(y, *linear_bound(x, w, s, None, group))
+    h = C.int4_gated_linear(x, w, w.flip(0), s, s, None, None, group)
+    _ok()
+    R.close_rounded(h, *R.gate_of(linear_bound(x, w, s, None, group), linear_bound(x, w.flip(0), s, None, group)))
 
 
 @pytest.mark.parametrize("M", [1, 8, 40])
@@ -192,8 +198,10 @@ def test_weight_past_32_bit_offsets():
         x = torch.randn(M, K, generator=g).half().to(DEV)
         y = C.int4_linear(x, w, s)
         _ok()
-        R.close_rounded(y[:, -16:], *linear_bound(x, R.unpack_int4(tail, st, K, 128), None))
-        assert (y[:, :-16] == 0).all()
+        R.close_rounded(y[:, -16:], *linear_bound(x, tail, st, None, 128))
+        # zeros, within the bound of a product whose parts are q + 8 and 8
+        zero, err = linear_bound(x, w[:1], s[:, :1], None, 128)
+        R.close_rounded(y[:, :-16], zero.expand(M, N - 16), err.expand(M, N - 16))
 
 
 def test_on_another_stream_and_in_a_graph():
@@ -295,14 +303,13 @@ def test_modules(dtype):
     m.bias.data.normal_()
     y = m(x)
     assert y.shape == (2, 3, 48) and y.dtype == x.dtype
-    want, err = R.linear(x.view(6, 264), R.unpack_int4(m.w_int4, m.w_scale, 264, 32), m.bias)
-    R.close_rounded(y.view(6, 48), want, err)
+    R.close_rounded(y.view(6, 48), *linear_bound(x.view(6, 264), m.w_int4, m.w_scale, m.bias, 32))
     gm = Int4GatedLinear(264, 48, group_size=32, dtype=TYPES[dtype]).to(DEV)
     gm.quantize_weight(w, w2)
     h = gm(x.transpose(0, 1))
-    want, err, _ = R.gate(x.transpose(0, 1).reshape(6, 264), R.unpack_int4(gm.w_gate_int4, gm.w_gate_scale, 264, 32),
-                          R.unpack_int4(gm.w_up_int4, gm.w_up_scale, 264, 32), None, None)
-    R.close_rounded(h.reshape(6, 48), want, err)
+    x2 = x.transpose(0, 1).reshape(6, 264)
+    R.close_rounded(h.reshape(6, 48), *R.gate_of(linear_bound(x2, gm.w_gate_int4, gm.w_gate_scale, None, 32),
+                                                 linear_bound(x2, gm.w_up_int4, gm.w_up_scale, None, 32)))
     other = Int4Linear(264, 48, group_size=32, dtype=TYPES[dtype]).to(DEV)
     other.load_state_dict(m.state_dict())
     assert torch.equal(other(x), y)

@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libforge_b200.so")
 SOURCES = ["capi.cu", "status.cu", "quantize.cu", "sparsity.cu", "gemm_dense.cu", "gemm_sparse.cu", "gemm_pair.cu", "gemm_fq.cu", "sparse_gemv.cu", "dense_gemv.cu", "probes.cu", "linear_static.cu", "conv.cu",
-           "int4.cu", "int4_stream.cu", "gated_stream.cu", "gated_linear.cu"]
+           "int4.cu", "int4_stream.cu", "int4_gemm.cu", "gated_stream.cu", "gated_linear.cu"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",

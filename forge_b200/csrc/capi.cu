@@ -54,6 +54,7 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, const __half*
 }
 
 inline bool is_16bit(int dtype) { return dtype == FORGE_DTYPE_F16 || dtype == FORGE_DTYPE_BF16; }
+constexpr int kInt4StreamTokens = 32;   // up to here one pass over 4-bit weights beats tensor-memory tiles
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline bool is_group(int g) { return g == 32 || g == 64 || g == 128; }
 
@@ -353,7 +354,7 @@ int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale,
         !aligned4(w_scale))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return int4_stream(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
+    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
                        dtype == FORGE_DTYPE_BF16, S(stream));
 }
 
@@ -368,7 +369,7 @@ int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t
         !aligned16(wu_int4) || !aligned4(wg_scale) || !aligned4(wu_scale))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return int4_stream(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
+    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
                        dtype == FORGE_DTYPE_BF16, S(stream));
 }
 

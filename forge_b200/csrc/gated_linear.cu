@@ -25,91 +25,24 @@
 #include "float_common.cuh"
 #include "gated_linear.cuh"
 #include "gemm_dense.cuh"
+#include "pair16.cuh"
 #include "ptx.cuh"
 
 namespace fb200 {
 
-using namespace ptx;
+using namespace pair16;
 
 namespace {
 
 constexpr int kThreads = 224;   // TMA warp (A), MMA warp, 4 epilogue warps, TMA warp (B)
-constexpr int kEpiWarps = 4;
-constexpr int kEpiThreads = 128;
-constexpr int kBand = 16;       // 256-row blocks of A per raster band
 
 enum Mode { kForward = 0, kForwardSave = 1, kDx = 2, kDw = 3 };
-
-struct Cfg {
-    static constexpr int kStages = 6;
-    static constexpr int kOperandBytes = 128 * 128;          // 128 rows (or channels) x 64 inputs of a CTA's half
-    static constexpr int kStageBytes = 2 * kOperandBytes;
-    static constexpr int kEpiBufs = 2;
-    static constexpr int kEpiBufBytes = 32 * 128;
-    static constexpr int kEpiBytes = kEpiWarps * kEpiBufs * kEpiBufBytes;
-    static constexpr int kBiasBytes = 2 * 256 * (int)sizeof(float);
-    static constexpr int kBarBytes = 256;
-    static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kBiasBytes + kBarBytes;
-    static constexpr int kTmemCols = 512;
-    static_assert(kSmemBytes <= 232448, "exceeds the 227 KB shared memory limit");
-};
-
-struct Bars {
-    uint64_t *full, *empty, *tmem_full, *tmem_empty;
-    uint32_t* tmem_slot;
-    volatile int* abort_flag;
-};
-__device__ __forceinline__ Bars carve(uint8_t* p) {
-    Bars b;
-    b.full = reinterpret_cast<uint64_t*>(p);      // in the leader: bytes of both CTAs' loads
-    b.empty = b.full + Cfg::kStages;              // one per CTA, committed by the leader's MMA thread
-    b.tmem_full = b.empty + Cfg::kStages;         // one per CTA
-    b.tmem_empty = b.tmem_full + 2;               // in the leader: both CTAs' epilogue warps
-    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + 2);
-    b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
-    return b;
-}
-
-// Instruction descriptor of kind::f16: fp32 accumulator, both operands fp16 or both bf16, each K-major or MN-major.
-__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a_mn, bool b_mn) {
-    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
-           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-        "}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// MN-major slab: chunks of 64 channels, each 64 rows (inputs) of 128 bytes with the 128-byte swizzle, 8 KB apart
-// (leading offset); groups of 8 inputs are 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr) {
-    return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | static_cast<uint64_t>(8192 >> 4) << 16 |
-           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
-}
 
 struct Maps {
     CUtensorMap a[2], b[2];   // operands of the first and second half of the work (see Mode)
     CUtensorMap out[2];       // h | dx | dWg, dWu
     CUtensorMap save[2];      // g, u (kForwardSave)
 };
-
-struct Tile {
-    int a_blk, b_blk;
-};
-__device__ __forceinline__ Tile tile_of(int t, int a_blocks, int b_blocks) {
-    const int band_tiles = kBand * b_blocks;
-    const int band = t / band_tiles;
-    const int rows = min(kBand, a_blocks - band * kBand);
-    const int r = t - band * band_tiles;
-    return {band * kBand + r % rows, r / rows};
-}
 
 // Rows (256 per tile) are tokens, or channels for kDw; columns are channels (kForward*: 128 per tile) or inputs.
 // rows, cols: extent of one output matrix; kb1: K blocks of the first operand pair, kbs: of both.
@@ -445,61 +378,16 @@ sum_parts_kernel(const float* __restrict__ part, T* __restrict__ dbg, T* __restr
 
 // ---------------------------------------------------------------------- host
 
-// (dim1, dim0) row-major elements, 128-byte wide swizzled boxes of `box_rows` rows; encoded anew in every call
-bool encode(CUtensorMap* m, CUtensorMapDataType type, int elem, const void* base, long long dim0, long long dim1,
-            int box_rows) {
-    PFN_encodeTiled fn = get_encode_fn();
-    if (fn == nullptr) return false;
-    const cuuint64_t dims[2] = {(cuuint64_t)dim0, (cuuint64_t)dim1};
-    const cuuint64_t strides[1] = {(cuuint64_t)dim0 * elem};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows};
-    const cuuint32_t es[2] = {1, 1};
-    return fn(m, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int MODE, bool BF16>
 int launch_pair(const Maps& maps, const void* bg, const void* bu, int rows, int cols, int kb1, int kbs,
                 cudaStream_t stream) {
     static int max_pairs[64] = {};
-    auto kern = gated_pair_kernel<MODE, BF16>;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int* status = status_word();
-    if (status == nullptr) return kLaunchFailed;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int& cap = max_pairs[dev & 63];
-    if (cap == 0) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes) != cudaSuccess)
-            return kLaunchFailed;
-        cfg.gridDim = dim3(2 * sm_count(), 1, 1);
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-            cudaGetLastError();
-            return kLaunchFailed;
-        }
-        cap = n;
-    }
     constexpr int TILE_N = MODE <= kForwardSave ? 128 : 256;
     const long long tiles = ((long long)rows + 255) / 256 * (MODE == kDw ? 2 : 1) * (((long long)cols + TILE_N - 1) / TILE_N);
-    if (tiles > 0x7fffffffll / 2) return kTooLarge;
-    cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, cap), 1, 1);
-    return cudaLaunchKernelEx(&cfg, kern, maps, bg, bu, rows, cols, kb1, kbs, status) == cudaSuccess ? kOk : kLaunchFailed;
-}
-
-CUtensorMapDataType type16(bool bf16) {
-    return bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    int* status = status_word();
+    if (status == nullptr) return kLaunchFailed;
+    return launch_pairs16(gated_pair_kernel<MODE, BF16>, kThreads, tiles, stream, max_pairs, maps, bg, bu, rows, cols, kb1,
+                          kbs, status);
 }
 
 inline size_t pad256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -531,10 +419,10 @@ int gated_linear(const void* x, const void* wg, const void* wu, const void* bg, 
     if (g == nullptr && M <= 16) return gated_stream(x, wg, wu, bg, bu, h, M, K, N, bf16, stream);
     Maps m = {};
     const CUtensorMapDataType t = type16(bf16), f = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    if (!encode(&m.a[0], t, 2, x, K, M, 128) || !encode(&m.b[0], t, 2, wg, K, N, 128) ||
-        !encode(&m.b[1], t, 2, wu, K, N, 128) || !encode(&m.out[0], t, 2, h, N, M, 32))
+    if (!encode_sw128(&m.a[0], t, 2, x, K, M, 128) || !encode_sw128(&m.b[0], t, 2, wg, K, N, 128) ||
+        !encode_sw128(&m.b[1], t, 2, wu, K, N, 128) || !encode_sw128(&m.out[0], t, 2, h, N, M, 32))
         return kLaunchFailed;
-    if (g != nullptr && (!encode(&m.save[0], f, 4, g, N, M, 32) || !encode(&m.save[1], f, 4, u, N, M, 32)))
+    if (g != nullptr && (!encode_sw128(&m.save[0], f, 4, g, N, M, 32) || !encode_sw128(&m.save[1], f, 4, u, N, M, 32)))
         return kLaunchFailed;
     const int kbs = (K + 63) / 64;
     if (g != nullptr)
@@ -561,9 +449,9 @@ int gated_linear_backward(const void* dh, const void* x, const void* wg, const v
     const CUtensorMapDataType t = type16(bf16);
     if (dx != nullptr) {
         Maps m = {};
-        if (!encode(&m.a[0], t, 2, dg, N, M, 128) || !encode(&m.a[1], t, 2, du, N, M, 128) ||
-            !encode(&m.b[0], t, 2, wg, K, N, 64) || !encode(&m.b[1], t, 2, wu, K, N, 64) ||
-            !encode(&m.out[0], t, 2, dx, K, M, 32))
+        if (!encode_sw128(&m.a[0], t, 2, dg, N, M, 128) || !encode_sw128(&m.a[1], t, 2, du, N, M, 128) ||
+            !encode_sw128(&m.b[0], t, 2, wg, K, N, 64) || !encode_sw128(&m.b[1], t, 2, wu, K, N, 64) ||
+            !encode_sw128(&m.out[0], t, 2, dx, K, M, 32))
             return kLaunchFailed;
         const int kb = (N + 63) / 64;
         r = bf16 ? launch_pair<kDx, true>(m, nullptr, nullptr, M, K, kb, 2 * kb, stream)
@@ -572,9 +460,9 @@ int gated_linear_backward(const void* dh, const void* x, const void* wg, const v
     }
     if (dwg != nullptr) {
         Maps m = {};
-        if (!encode(&m.a[0], t, 2, dg, N, M, 64) || !encode(&m.a[1], t, 2, du, N, M, 64) ||
-            !encode(&m.b[0], t, 2, x, K, M, 64) || !encode(&m.out[0], t, 2, dwg, K, N, 32) ||
-            !encode(&m.out[1], t, 2, dwu, K, N, 32))
+        if (!encode_sw128(&m.a[0], t, 2, dg, N, M, 64) || !encode_sw128(&m.a[1], t, 2, du, N, M, 64) ||
+            !encode_sw128(&m.b[0], t, 2, x, K, M, 64) || !encode_sw128(&m.out[0], t, 2, dwg, K, N, 32) ||
+            !encode_sw128(&m.out[1], t, 2, dwu, K, N, 32))
             return kLaunchFailed;
         const int kb = (M + 63) / 64;
         r = bf16 ? launch_pair<kDw, true>(m, nullptr, nullptr, N, K, kb, kb, stream)

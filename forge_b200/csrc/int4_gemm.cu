@@ -1,0 +1,454 @@
+// Linear layers on 4-bit weights for many tokens: CTA-pair tcgen05 GEMM (cta_group::2, kind::f16) whose weight operand
+// is made in the kernel.
+//
+//   plain:  out[m][n] = sum_k x[m][k] w[n][k] + b[n]            w[n][k] = s[k / G][n] q[n][k]
+//   gated:  out[m][n] = SiLU(g) u, g = x Wg^T + bg, u = x Wu^T + bu
+//
+// The skeleton of the other pair kernels (256 tokens x BN weight rows per pair), with the weight's TMA producer replaced by
+// twelve warps per CTA that read packed weights from L2, multiply the integers by their scales and write 16-bit numbers
+// in the swizzled layout that the tensor cores read; nothing of the unpacked weight ever reaches memory. Gated, CTA 0
+// makes rows of Wg and CTA 1 the same rows of Wu. A stage is a whole block of 128 inputs (three of 64 KB). Making one takes
+// longer than the tensor cores need for it, so each stage has four warps of its own, three blocks being made at a time; the
+// warps signal a barrier of their own CTA only, and one thread passes CTA 1's on to the leader (with eight warps on each
+// 64-deep slab in turn and arrivals across the cluster, 2048 x 4096 x 11008 took 308 us).
+//
+// A weight is rounded once, to the activations' type, as s q: exactly the product of the two, rounded (bf16: s is split
+// into two bf16 numbers whose products with q are exact, so that one fused multiply-add rounds their sum). That is one
+// rounding more than the few-token kernel has; accumulators are fp32.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "float_common.cuh"
+#include "gemm_dense.cuh"
+#include "int4.cuh"
+#include "pair16.cuh"
+#include "ptx.cuh"
+
+namespace fb200 {
+
+using namespace pair16;
+
+namespace {
+
+constexpr int kRing = 3;          // stages: two 64-deep slabs of both operands each
+constexpr int kGroupWarps = 4;    // that make a stage's weights
+constexpr int kWeightWarps = kRing * kGroupWarps;
+constexpr int kSlab = Cfg::kOperandBytes;
+
+struct RingBars {
+    uint64_t *full, *empty, *made, *tmem_full, *tmem_empty;
+    uint32_t* tmem_slot;
+    volatile int* abort_flag;
+};
+__device__ __forceinline__ RingBars carve_ring(uint8_t* p) {
+    RingBars b;
+    b.full = reinterpret_cast<uint64_t*>(p);   // in the leader: both CTAs' activations, its weight warps, CTA 1's relay
+    b.empty = b.full + kRing;                  // one per CTA, committed by the leader's MMA thread
+    b.made = b.empty + kRing;                  // in CTA 1: its weight warps
+    b.tmem_full = b.made + kRing;              // one per CTA
+    b.tmem_empty = b.tmem_full + 2;            // in the leader: both CTAs' epilogue warps
+    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + 2);
+    b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
+    return b;
+}
+constexpr int kThreads = 32 * (2 + kEpiWarps + kWeightWarps);   // TMA warp, MMA warp, epilogue, weights
+
+// Word of 8 four-bit weights times its scale -> 8 numbers of type T in order. A nibble in the low mantissa bits of 1024
+// (fp16) or 128 (bf16) is that number plus the nibble, exactly; subtracting the offset + 8 leaves q, exactly.
+template <typename T>
+struct Scaled;
+template <>
+struct Scaled<__half> {
+    __half2 s;
+    __device__ __forceinline__ explicit Scaled(unsigned short bits) : s(__half2half2(__ushort_as_half(bits))) {}
+    __device__ __forceinline__ uint4 operator()(uint32_t w) const {
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t v = w >> (8 * i);
+            const uint32_t lo = and_or(v, 0x000F000Fu, 0x64006400u), hi = and_or(v, 0x00F000F0u, 0x64006400u);
+            const __half2 a = __hsub2(reinterpret_cast<const __half2&>(lo), __half2half2(__ushort_as_half(0x6408)));
+            const __half2 b = __hfma2(reinterpret_cast<const __half2&>(hi), __half2half2(__ushort_as_half(0x2C00)),
+                                      __half2half2(__ushort_as_half(0xD480)));   // / 16 - 72
+            const __half2 x = __hmul2(a, s), y = __hmul2(b, s);
+            f[2 * i] = reinterpret_cast<const uint32_t&>(x);
+            f[2 * i + 1] = reinterpret_cast<const uint32_t&>(y);
+        }
+        return make_uint4(f[0], f[1], f[2], f[3]);
+    }
+};
+template <>
+struct Scaled<__nv_bfloat16> {
+    __nv_bfloat162 hi, lo;
+    __device__ __forceinline__ explicit Scaled(unsigned short bits) {
+        const float s = __half2float(__ushort_as_half(bits));
+        const __nv_bfloat16 h = __float2bfloat16_rn(s);
+        hi = __bfloat162bfloat162(h);
+        lo = __bfloat162bfloat162(__float2bfloat16_rn(s - __bfloat162float(h)));
+    }
+    __device__ __forceinline__ uint4 operator()(uint32_t w) const {
+        uint32_t f[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+            const __nv_bfloat162 q =
+                __hsub2(reinterpret_cast<const __nv_bfloat162&>(b), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
+            const __nv_bfloat162 v = __hfma2(q, hi, __hmul2(q, lo));
+            f[i] = reinterpret_cast<const uint32_t&>(v);
+        }
+        return make_uint4(f[0], f[1], f[2], f[3]);
+    }
+};
+
+// BN: weight rows per tile (256 or 128), of both matrices when GATED.
+template <typename T, int G, bool GATED, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
+                 const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1, const __half* __restrict__ s0,
+                 const __half* __restrict__ s1, const T* __restrict__ b0, const T* __restrict__ b1, T* __restrict__ out,
+                 int M, int N, int K, int tma_out, int* __restrict__ status) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int TILE_N = GATED ? BN / 2 : BN;   // output columns
+    constexpr int HALF = BN / 2;                  // weight rows that a CTA makes
+    constexpr int PER = 128 / G;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    static_assert(kRing * 4 * kSlab == Cfg::kStages * Cfg::kStageBytes, "the shared-memory plan of Cfg");
+    uint8_t* smem_epi = smem + kRing * 4 * kSlab;   // a stage: activations of both slabs, weights of both
+    float* smem_bias = reinterpret_cast<float*>(smem_epi + Cfg::kEpiBytes);
+    const RingBars bars = carve_ring(smem_epi + Cfg::kEpiBytes + Cfg::kBiasBytes);
+
+    const int warp_id = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    if ((smem_u32(smem) & 1023u) != 0) {   // the same in both CTAs
+        if (threadIdx.x == 0) atomicExch(status, 850);
+        return;
+    }
+    const int a_blocks = (M + 255) / 256, b_blocks = (N + TILE_N - 1) / TILE_N;
+    const int num_tiles = a_blocks * b_blocks;
+    const int blocks = (K + 127) / 128;
+    const int pair_id = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kRing; s++) {
+            mbar_init(&bars.full[s], 1 + kGroupWarps + 1);
+            mbar_init(&bars.empty[s], 1);
+            mbar_init(&bars.made[s], kGroupWarps);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.tmem_full[i], 1);
+            mbar_init(&bars.tmem_empty[i], 2 * kEpiWarps);
+        }
+        *bars.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp_id == 1) {
+        tmem_alloc_pair(bars.tmem_slot, Cfg::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers are initialised before anything signals them
+    tc_fence_after();
+    const uint32_t tmem_base = *bars.tmem_slot;
+
+    if (warp_id == 0) {
+        // ------------------------------------------------------------------ activations (TMA)
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair_id; t < num_tiles && ok; t += num_pairs) {
+                const Tile tc = tile_of(t, a_blocks, b_blocks);
+                for (int blk = 0; blk < blocks; blk++) {
+                    if (!mbar_wait(&bars.empty[stage], phase ^ 1, bars.abort_flag)) {
+                        atomicExch(status, 851);
+                        ok = false;
+                        break;
+                    }
+                    if (leader) mbar_expect_tx(&bars.full[stage], 4 * kSlab);
+                    const uint32_t full = mapa_shared(smem_u32(&bars.full[stage]), 0);
+                    uint8_t* dst = smem + stage * 4 * kSlab;
+                    tma_load_2d_pair(dst, &tm_x, full, blk * 128, tc.a_blk * 256 + (int)rank * 128);
+                    tma_load_2d_pair(dst + kSlab, &tm_x, full, blk * 128 + 64, tc.a_blk * 256 + (int)rank * 128);
+                    if (++stage == kRing) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp_id == 1) {
+        // ------------------------------------------------------------------ MMA issuer (leader only)
+        if (leader && lane == 0) {
+            constexpr uint32_t idesc = idesc_f16(256, BN, BF16, false, false);
+            int stage = 0;
+            uint32_t phase = 0;
+            int local = 0;
+            bool ok = true;
+            for (int t = pair_id; t < num_tiles && ok; t += num_pairs, local++) {
+                const int buf = local & 1;
+                if (!mbar_wait(&bars.tmem_empty[buf], ((local >> 1) & 1) ^ 1, bars.abort_flag)) {
+                    atomicExch(status, 852);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem_base + buf * 256;
+                for (int blk = 0; blk < blocks; blk++) {
+                    // cluster scope: the other CTA's relay signals this barrier with a plain arrival
+                    if (!mbar_wait_cluster(&bars.full[stage], phase, bars.abort_flag)) {
+                        atomicExch(status, 853);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + stage * 4 * kSlab);
+                    const uint64_t da = make_desc_sw128(sa), db = make_desc_sw128(sa + 2 * kSlab);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int step = (k / 4) * (kSlab >> 4) + 2 * (k % 4);
+                        umma_f16_pair(acc, da + step, db + step, idesc, (blk | k) != 0 ? 1u : 0u);
+                    }
+                    tc_commit_pair_mask(smem_u32(&bars.empty[stage]), 3);
+                    if (++stage == kRing) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok) tc_commit_pair_mask(smem_u32(&bars.tmem_full[buf]), 3);
+            }
+        } else if (!leader && lane == 0) {
+            // relay: this CTA's half of a stage's weights is there
+            int stage = 0;
+            uint32_t phase = 0;
+            const long long turns = (long long)((num_tiles - pair_id + num_pairs - 1) / num_pairs) * blocks;
+            for (long long i = 0; i < turns; i++) {
+                if (!mbar_wait(&bars.made[stage], phase, bars.abort_flag)) {
+                    atomicExch(status, 856);
+                    break;
+                }
+                mbar_arrive_cluster(mapa_shared(smem_u32(&bars.full[stage]), 0));
+                if (++stage == kRing) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp_id >= 2 + kEpiWarps) {
+        // ------------------------------------------------------------------ weights (both CTAs)
+        // A lane makes a quarter (16 packed bytes: runs t, 4 + t, 8 + t, 12 + t) of a block of two or four rows. Rows go to
+        // lanes so that eight lanes write all banks.
+        constexpr int ROWS = HALF / (8 * kGroupWarps);
+        const int t4 = lane & 3;
+        const int row8 = (lane >> 3) | ((lane >> 2) & 1) << 2;
+        const int group = (warp_id - 2 - kEpiWarps) / kGroupWarps;
+        const int local_row = (warp_id - 2 - kEpiWarps) % kGroupWarps * 8 + row8;
+        const uint8_t* w = GATED && rank == 1 ? w1 : w0;
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(GATED && rank == 1 ? s1 : s0);
+        const int groups = (K + G - 1) / G;
+        // Every third block of those that the CTA goes through, always into the same stage: a barrier's parity tells a lap
+        // from its neighbours only, so whoever waits on it has to see every lap.
+        const int stage = group;
+        uint32_t phase = 0;
+        bool ok = true;
+        int blk = group;     // in its tile
+        for (int t = pair_id; t < num_tiles && ok; t += num_pairs) {
+            const Tile tc = tile_of(t, a_blocks, b_blocks);
+            const uint8_t* wp[ROWS];
+            int row[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) {
+                row[i] = min(tc.b_blk * TILE_N + (GATED ? 0 : (int)rank * HALF) + local_row + 8 * kGroupWarps * i, N - 1);
+                wp[i] = w + (size_t)row[i] * ((size_t)blocks * 64) + t4 * 16;
+            }
+            uint4 next[ROWS];
+            unsigned short next_s[ROWS][PER];
+            auto load = [&](int b) {
+#pragma unroll
+                for (int i = 0; i < ROWS; i++) {
+                    next[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
+#pragma unroll
+                    for (int k = 0; k < PER; k++) next_s[i][k] = __ldg(s + (size_t)min(b * PER + k, groups - 1) * N + row[i]);
+                }
+            };
+            if (blk < blocks) load(blk);
+            for (; blk < blocks; blk += kRing) {
+                uint4 cur[ROWS];
+                unsigned short cur_s[ROWS][PER];
+#pragma unroll
+                for (int i = 0; i < ROWS; i++) {
+                    cur[i] = next[i];
+#pragma unroll
+                    for (int k = 0; k < PER; k++) cur_s[i][k] = next_s[i][k];
+                }
+                load(min(blk + kRing, blocks - 1));
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty[stage], phase ^ 1, bars.abort_flag));
+                if (!ok) {
+                    if (lane == 0) atomicExch(status, 854);
+                    break;
+                }
+                phase ^= 1;
+                uint8_t* dst = smem + stage * 4 * kSlab + 2 * kSlab + local_row * 128;
+#pragma unroll
+                for (int i = 0; i < ROWS; i++) {
+                    const uint32_t word[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (8 * kGroupWarps * 128) +
+                                                  (((4 * (j % 2) + t4) ^ row8) << 4)) =
+                            Scaled<T>(cur_s[i][j * 32 / G])(word[j]);
+                }
+                fence_proxy_async_smem();   // the tensor cores read through the async proxy
+                __syncwarp();
+                if (lane == 0) mbar_arrive(leader ? &bars.full[stage] : &bars.made[stage]);
+            }
+            blk -= blocks;
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue (both CTAs)
+        const int q = warp_id & 3;
+        const int epi_tid = (warp_id - 2) * 32 + lane;
+        uint8_t* my_stage = smem_epi + (warp_id - 2) * Cfg::kEpiBufs * Cfg::kEpiBufBytes;
+        const uint64_t policy = l2_policy_evict_first();   // outputs must not push operands out of L2
+        int sbuf = 0, local = 0;
+        bool ok = true;
+        for (int t = pair_id; t < num_tiles; t += num_pairs, local++) {
+            const Tile tc = tile_of(t, a_blocks, b_blocks);
+            const int buf = local & 1;
+            const int row0 = tc.a_blk * 256 + (int)rank * 128 + q * 32;
+            const int n0 = tc.b_blk * TILE_N;
+            float* bias = smem_bias + buf * 256;   // TILE_N of b0; gated: then TILE_N of b1
+            for (int i = epi_tid; i < BN; i += kEpiThreads) {
+                const int n = n0 + i % TILE_N;
+                const T* b = i < TILE_N ? b0 : b1;
+                bias[i] = b != nullptr && n < N ? to_float(b[n]) : 0.f;
+            }
+            named_barrier_sync(1, kEpiThreads);
+            if (ok) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[buf], (local >> 1) & 1, bars.abort_flag));
+                if (!ok) atomicExch(status, 855);
+            }
+            if (!ok) continue;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
+#pragma unroll 1
+            for (int c = 0; c < TILE_N / 64; c++) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    const int col = c * 64 + hh * 32;
+                    uint32_t va[32], vb[32];
+                    tmem_ld_32x32b_x32(taddr + col, va);
+                    if (GATED) tmem_ld_32x32b_x32(taddr + TILE_N + col, vb);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        float o[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            o[e] = __uint_as_float(va[2 * i + e]) + bias[col + 2 * i + e];
+                            if (GATED) o[e] = silu_mul(o[e], __uint_as_float(vb[2 * i + e]) + bias[TILE_N + col + 2 * i + e]);
+                        }
+                        packed[hh * 16 + i] = pack2<T>(o[0], o[1]);
+                    }
+                }
+                if (row0 >= M || n0 + c * 64 >= N) continue;   // nothing to store; a box must not start outside
+                uint8_t* stg = my_stage + sbuf * Cfg::kEpiBufBytes;
+                if (lane == 0) tma_store_wait_read<Cfg::kEpiBufs - 1>();
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    *reinterpret_cast<uint4*>(stg + lane * 128 + (j ^ (lane & 7)) * 16) =
+                        make_uint4(packed[4 * j], packed[4 * j + 1], packed[4 * j + 2], packed[4 * j + 3]);
+                if (tma_out) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d_hint(&tm_out, stg, n0 + c * 64, row0, policy);
+                        tma_store_commit();
+                    }
+                } else {   // rows that are no multiple of 16 bytes: two neighbouring columns a lane, row after row
+                    __syncwarp();
+                    const int n = n0 + c * 64 + 2 * lane;
+                    for (int r = 0; r < 32 && row0 + r < M; r++) {
+                        const T* v = reinterpret_cast<const T*>(stg + r * 128 + ((lane >> 2) ^ (r & 7)) * 16 + (lane & 3) * 4);
+                        T* o = out + (size_t)(row0 + r) * N + n;
+                        if (n < N) o[0] = v[0];
+                        if (n + 1 < N) o[1] = v[1];
+                    }
+                }
+                sbuf = (sbuf + 1) % Cfg::kEpiBufs;
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote_cta_scope(mapa_shared(smem_u32(&bars.tmem_empty[buf]), 0));
+        }
+        if (lane == 0) tma_store_wait_all<0>();
+    }
+
+    // ---------------------------------------------------------------------- teardown
+    if (*bars.abort_flag != 0) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) { }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // neither CTA frees TMEM or exits while the peer can still touch it
+    if (warp_id == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    }
+}
+
+template <typename T, int G, bool GATED, int BN>
+int launch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
+           const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
+    static int max_pairs[64] = {};
+    constexpr int TILE_N = GATED ? BN / 2 : BN;
+    const CUtensorMapDataType type = type16(std::is_same<T, __nv_bfloat16>::value);
+    const int tma_out = N % 8 == 0 && aligned16(out);
+    CUtensorMap tm_x, tm_out;
+    if (!encode_sw128(&tm_x, type, 2, x, K, M, 128)) return kLaunchFailed;
+    tm_out = tm_x;
+    if (tma_out && !encode_sw128(&tm_out, type, 2, out, N, M, 32)) return kLaunchFailed;
+    int* status = status_word();
+    if (status == nullptr) return kLaunchFailed;
+    const long long tiles = ((long long)M + 255) / 256 * (((long long)N + TILE_N - 1) / TILE_N);
+    return launch_pairs16(int4_pair_kernel<T, G, GATED, BN>, kThreads, tiles, stream, max_pairs, tm_x, tm_out, w0, w1, s0, s1,
+                          static_cast<const T*>(b0), static_cast<const T*>(b1), static_cast<T*>(out), M, N, K, tma_out,
+                          status);
+}
+
+template <typename T, int G>
+int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
+             const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
+    const bool gated = w1 != nullptr;
+    // 128 weight rows a tile take 0.6 of the time of 256 (tensor instructions of 128 columns run at their floor of 86
+    // clocks): where even those leave pairs without a tile
+    const long long wide = ((long long)M + 255) / 256 * (((long long)N * (gated ? 2 : 1) + 255) / 256);
+    if (2 * wide <= sm_count() / 2)
+        return gated ? launch<T, G, true, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                     : launch<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    return gated ? launch<T, G, true, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                 : launch<T, G, false, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+}
+
+}  // namespace
+
+int int4_gemm(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
+              const void* b1, void* out, int M, int K, int N, int group, bool bf16, cudaStream_t st) {
+    switch (group * 2 + (bf16 ? 1 : 0)) {
+    case 64: return dispatch<__half, 32>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    case 65: return dispatch<__nv_bfloat16, 32>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    case 128: return dispatch<__half, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    case 129: return dispatch<__nv_bfloat16, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    case 256: return dispatch<__half, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    case 257: return dispatch<__nv_bfloat16, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    default: return kBadShape;
+    }
+}
+
+}  // namespace fb200

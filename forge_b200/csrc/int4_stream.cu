@@ -34,13 +34,6 @@ constexpr int kWarps = 8;
 constexpr int kRing = 6;              // KB of a warp's weights under way: 6 * 24 warps, and room for activations in L1
 constexpr int kTokStride = 20;        // floats per token of a partial sum: 16 rows + 4, conflict-free fragment writes
 
-// (v & mask) | bits in one instruction
-__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
-    return r;
-}
-
 // Word of 8 four-bit weights (weight 2i in nibble i, weight 2i + 1 in nibble i + 4, stored as the integer + 8) -> four
 // pairs of 16-bit floats, the first two for one accumulator (A), the others for another (B); their sum is A + B * kB.
 //   fp16: a nibble alone in a half is the subnormal number n 2^-24, or 16 n 2^-24 where it lies four bits up; tensor

@@ -246,7 +246,7 @@ int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, vo
                               int group_size, forge_stream_t stream);
 
 /* output (M,N) = x (M,K) W^T + bias (N, may be NULL); x, bias and output of `dtype` (FORGE_DTYPE_F16 or _BF16). Sums in
- * fp32, one rounding at the end. Needs K % 8 == 0, 16-byte aligned x and w_int4, 4-byte aligned w_scale
+ * fp32, one rounding at the end; with more than 32 tokens scale * q is first rounded to `dtype` (it must be in its range). Needs K % 8 == 0, 16-byte aligned x and w_int4, 4-byte aligned w_scale
  * (FORGE_B200_BAD_SHAPE otherwise). */
 int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale, const void* bias, void* output, int M,
                       int K, int N, int group_size, int dtype, forge_stream_t stream);
@@ -321,8 +321,8 @@ int forge_int8_conv_transpose2d_k2s2_forward(const void* input, const int8_t* we
  * cannot be read). forge_b200_device_status_raw returns the recorded code itself:
  *   100-104 dense GEMM, 200-204 2:4-sparse GEMM, 300-304 / 400-404 their CTA-pair forms,
  *   500-506 fused quantize + sparse GEMM, 600-605 convolution, 700-704 gated linear layer on 16-bit
- *   weights, 800-801 weight streaming for few tokens on 4-bit or 16-bit weights; within a range x00 = misaligned
- *   shared memory, x01 = producer waiting for a free stage, x02 = MMA issuer waiting for a drained
+ *   weights, 800-801 its few-token form, 850-856 4-bit GEMM; within a range x00 = misaligned shared
+ *   memory, x01 = producer waiting for a free stage, x02 = MMA issuer waiting for a drained
  *   accumulator, x03 = MMA issuer waiting for operands, x04 and up = epilogue / gather waits.
  * Both synchronise the device; reset != 0 clears the word after reading it. */
 int forge_b200_device_status(int reset);

@@ -54,7 +54,7 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, const __half*
 }
 
 inline bool is_16bit(int dtype) { return dtype == FORGE_DTYPE_F16 || dtype == FORGE_DTYPE_BF16; }
-constexpr int kInt4StreamTokens = 32;   // up to here one pass over 4-bit weights beats tensor-memory tiles
+constexpr int kInt4StreamTokens = 8;    // up to here one pass over 4-bit weights beats tensor-memory tiles
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline bool is_group(int g) { return g == 32 || g == 64 || g == 128; }
 

@@ -35,6 +35,7 @@ constexpr int kRing = 3;          // stages: two 64-deep slabs of both operands 
 constexpr int kGroupWarps = 4;    // that make a stage's weights
 constexpr int kWeightWarps = kRing * kGroupWarps;
 constexpr int kSlab = Cfg::kOperandBytes;
+constexpr int kTokensMax = 128;   // tokens up to which weight rows are the tensor cores' lanes
 
 struct RingBars {
     uint64_t *full, *empty, *made, *tmem_full, *tmem_empty;
@@ -100,6 +101,23 @@ struct Scaled<__nv_bfloat16> {
         return make_uint4(f[0], f[1], f[2], f[3]);
     }
 };
+
+// One thread of CTA 1: tells the leader, stage after stage, that CTA 1's half of the weights is there.
+__device__ __forceinline__ void relay(const RingBars& bars, long long turns, int* status) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (long long i = 0; i < turns; i++) {
+        if (!mbar_wait(&bars.made[stage], phase, bars.abort_flag)) {
+            atomicExch(status, 856);
+            return;
+        }
+        mbar_arrive_cluster(mapa_shared(smem_u32(&bars.full[stage]), 0));
+        if (++stage == kRing) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+}
 
 // BN: weight rows per tile (256 or 128), of both matrices when GATED.
 template <typename T, int G, bool GATED, int BN>
@@ -221,21 +239,7 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 if (ok) tc_commit_pair_mask(smem_u32(&bars.tmem_full[buf]), 3);
             }
         } else if (!leader && lane == 0) {
-            // relay: this CTA's half of a stage's weights is there
-            int stage = 0;
-            uint32_t phase = 0;
-            const long long turns = (long long)((num_tiles - pair_id + num_pairs - 1) / num_pairs) * blocks;
-            for (long long i = 0; i < turns; i++) {
-                if (!mbar_wait(&bars.made[stage], phase, bars.abort_flag)) {
-                    atomicExch(status, 856);
-                    break;
-                }
-                mbar_arrive_cluster(mapa_shared(smem_u32(&bars.full[stage]), 0));
-                if (++stage == kRing) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            }
+            relay(bars, (long long)((num_tiles - pair_id + num_pairs - 1) / num_pairs) * blocks, status);
         }
     } else if (warp_id >= 2 + kEpiWarps) {
         // ------------------------------------------------------------------ weights (both CTAs)
@@ -403,6 +407,328 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
     }
 }
 
+// Up to 128 tokens: the operands change places. Weight rows are the lanes, tokens the columns, as many as there are (`cols`,
+// a multiple of 16), so the tensor instructions shrink with the batch, and what bounds the call is how fast weights become
+// operands. One CTA per tile of `rows` rows (gated: of each matrix, Wg in lanes 0-63 and Wu in lanes 64-127), chosen so
+// that all SMs have the same number; rows beyond it are stale shared memory in accumulator lanes of their own, not stored.
+// Weights and activations have rings of their own: a weight stage (32 KB) is made within half a microsecond of being
+// free, while a copy of activations takes a whole one (one ring of three for both, on CTA pairs: 33 us for every batch).
+struct TokenBars {
+    uint64_t *full_w, *empty_w;   // [kRing]: the stage's weight warps; committed by the MMA thread
+    uint64_t *full_x, *empty_x;   // [kMaxRingX]
+    uint64_t *tmem_full, *tmem_empty;
+    uint32_t* tmem_slot;
+    volatile int* abort_flag;
+};
+constexpr int kMaxRingX = 8;
+constexpr int kSwapBytes = 32 * 64 * 4;   // gated: the up products of 32 tokens x 64 rows
+__device__ __forceinline__ TokenBars carve_tokens(uint8_t* p) {
+    TokenBars b;
+    b.full_w = reinterpret_cast<uint64_t*>(p);
+    b.empty_w = b.full_w + kRing;
+    b.full_x = b.empty_w + kRing;
+    b.empty_x = b.full_x + kMaxRingX;
+    b.tmem_full = b.empty_x + kMaxRingX;
+    b.tmem_empty = b.tmem_full + 2;
+    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + 2);
+    b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
+    return b;
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <typename T, int G, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
+                   const __half* __restrict__ s0, const __half* __restrict__ s1, const T* __restrict__ b0,
+                   const T* __restrict__ b1, T* __restrict__ out, int M, int N, int K, int rows, int cols, int ring_x,
+                   int* __restrict__ status) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr int PER = 128 / G;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int slab_x = cols * 128;
+    uint8_t* smem_x = smem + kRing * 2 * kSlab;
+    uint8_t* smem_swap = smem_x + ring_x * 2 * slab_x;
+    const TokenBars bars = carve_tokens(smem_swap + kSwapBytes);
+
+    const int warp_id = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if ((smem_u32(smem) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicExch(status, 850);
+        return;
+    }
+    const int num_tiles = (N + rows - 1) / rows;
+    const int blocks = (K + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kRing; s++) {
+            mbar_init(&bars.full_w[s], kGroupWarps);
+            mbar_init(&bars.empty_w[s], 1);
+        }
+        for (int s = 0; s < ring_x; s++) {
+            mbar_init(&bars.full_x[s], 1);
+            mbar_init(&bars.empty_x[s], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.tmem_full[i], 1);
+            mbar_init(&bars.tmem_empty[i], kEpiWarps);
+        }
+        *bars.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp_id == 1) {
+        tmem_alloc(bars.tmem_slot, 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *bars.tmem_slot;
+
+    if (warp_id == 0) {
+        // ------------------------------------------------------------------ activations (TMA)
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+                for (int blk = 0; blk < blocks; blk++) {
+                    if (!mbar_wait(&bars.empty_x[stage], phase ^ 1, bars.abort_flag)) {
+                        atomicExch(status, 851);
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = smem_x + stage * 2 * slab_x;
+                    mbar_expect_tx(&bars.full_x[stage], 2 * slab_x);
+                    tma_load_2d(dst, &tm_x, &bars.full_x[stage], blk * 128, 0);
+                    tma_load_2d(dst + slab_x, &tm_x, &bars.full_x[stage], blk * 128 + 64, 0);
+                    if (++stage == ring_x) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp_id == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            const uint32_t idesc = idesc_f16(128, cols, BF16, false, false);
+            int stage = 0, stage_x = 0, local = 0;
+            uint32_t phase = 0, phase_x = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, local++) {
+                const int buf = local & 1;
+                if (!mbar_wait(&bars.tmem_empty[buf], ((local >> 1) & 1) ^ 1, bars.abort_flag)) {
+                    atomicExch(status, 852);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem_base + buf * 128;
+                for (int blk = 0; blk < blocks; blk++) {
+                    if (!mbar_wait(&bars.full_x[stage_x], phase_x, bars.abort_flag) ||
+                        !mbar_wait(&bars.full_w[stage], phase, bars.abort_flag)) {
+                        atomicExch(status, 853);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = make_desc_sw128(smem_u32(smem + stage * 2 * kSlab));
+                    const uint64_t db = make_desc_sw128(smem_u32(smem_x + stage_x * 2 * slab_x));
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        umma_f16(acc, da + (k / 4) * (kSlab >> 4) + 2 * (k % 4), db + (k / 4) * (slab_x >> 4) + 2 * (k % 4),
+                                 idesc, (blk | k) != 0 ? 1u : 0u);
+                    tc_commit(&bars.empty_w[stage]);
+                    tc_commit(&bars.empty_x[stage_x]);
+                    if (++stage == kRing) {
+                        stage = 0;
+                        phase ^= 1;
+                    }
+                    if (++stage_x == ring_x) {
+                        stage_x = 0;
+                        phase_x ^= 1;
+                    }
+                }
+                if (ok) tc_commit(&bars.tmem_full[buf]);
+            }
+        }
+    } else if (warp_id >= 2 + kEpiWarps) {
+        // ------------------------------------------------------------------ weights, as in int4_pair_kernel
+        constexpr int ROWS = 4;   // of a lane; the last ones only where a CTA has so many
+        const int t4 = lane & 3;
+        const int row8 = (lane >> 3) | ((lane >> 2) & 1) << 2;
+        const int group = (warp_id - 2 - kEpiWarps) / kGroupWarps;
+        const int local_row = (warp_id - 2 - kEpiWarps) % kGroupWarps * 8 + row8;
+        const int groups = (K + G - 1) / G;
+        const int stage = group;
+        uint32_t phase = 0;
+        bool ok = true;
+        int blk = group;
+        // i-th row of a lane: i * 32 + local_row (gated: rows 0-31 and 32-63 of Wg, then of Wu)
+        auto used = [&](int i) { return (GATED ? i % 2 : i) * 8 * kGroupWarps < rows; };
+        for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+            const uint8_t* wp[ROWS];
+            const unsigned short* sp[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) {
+                const bool second = GATED && i >= ROWS / 2;
+                const int row = min(t * rows + (GATED ? i % 2 : i) * 8 * kGroupWarps + local_row, N - 1);
+                wp[i] = (second ? w1 : w0) + (size_t)row * ((size_t)blocks * 64) + t4 * 16;
+                sp[i] = reinterpret_cast<const unsigned short*>(second ? s1 : s0) + row;
+            }
+            uint4 next[2][ROWS];   // of the stage's next block and the one behind it
+            unsigned short next_s[2][ROWS][PER];
+            auto load = [&](int b, uint4 (&v)[ROWS], unsigned short (&sc)[ROWS][PER]) {
+#pragma unroll
+                for (int i = 0; i < ROWS; i++)
+                    if (used(i)) {
+                        v[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
+#pragma unroll
+                        for (int k = 0; k < PER; k++) sc[i][k] = __ldg(sp[i] + (size_t)min(b * PER + k, groups - 1) * N);
+                    }
+            };
+            auto make = [&](uint4 (&v)[ROWS], unsigned short (&sc)[ROWS][PER]) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty_w[stage], phase ^ 1, bars.abort_flag));
+                if (!ok) {
+                    if (lane == 0) atomicExch(status, 854);
+                    return;
+                }
+                phase ^= 1;
+                uint8_t* dst = smem + stage * 2 * kSlab + local_row * 128;
+#pragma unroll
+                for (int i = 0; i < ROWS; i++)
+                    if (used(i)) {
+                        const uint32_t word[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (8 * kGroupWarps * 128) +
+                                                      (((4 * (j % 2) + t4) ^ row8) << 4)) = Scaled<T>(sc[i][j * 32 / G])(word[j]);
+                    }
+                fence_proxy_async_smem();   // the tensor cores read through the async proxy
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.full_w[stage]);
+            };
+            load(min(blk, blocks - 1), next[0], next_s[0]);
+            load(min(blk + kRing, blocks - 1), next[1], next_s[1]);
+            while (blk < blocks && ok) {
+                make(next[0], next_s[0]);
+                load(min(blk + 2 * kRing, blocks - 1), next[0], next_s[0]);
+                blk += kRing;
+                if (blk >= blocks || !ok) break;
+                make(next[1], next_s[1]);
+                load(min(blk + 2 * kRing, blocks - 1), next[1], next_s[1]);
+                blk += kRing;
+            }
+            blk -= blocks;
+        }
+    } else {
+        // ------------------------------------------------------------------ epilogue: a lane has a row's products with all tokens
+        const int q = warp_id & 3;
+        float* swap = reinterpret_cast<float*>(smem_swap);
+        int local = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, local++) {
+            const int buf = local & 1;
+            const int r = GATED ? (q % 2) * 32 + lane : q * 32 + lane;
+            const int n = t * rows + r;
+            const bool live = r < rows && n < N;
+            const T* b = GATED && q >= 2 ? b1 : b0;
+            const float bias = live && b != nullptr ? to_float(b[n]) : 0.f;
+            if (ok) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[buf], (local >> 1) & 1, bars.abort_flag));
+                if (!ok && lane == 0) atomicExch(status, 855);
+            }
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * 128;
+#pragma unroll 1
+            for (int c = 0; c < (cols + 31) / 32; c++) {
+                uint32_t v[32];
+                if (ok) {
+                    tmem_ld_32x32b_x32(taddr + c * 32, v);
+                    tmem_ld_wait();
+                }
+                if constexpr (GATED) {
+                    if (q >= 2 && ok) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) swap[i * 64 + r] = __uint_as_float(v[i]) + bias;
+                    }
+                    named_barrier_sync(1, kEpiThreads);
+                    if (q < 2 && ok) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const int m = c * 32 + i;
+                            if (live && m < M)
+                                out[(size_t)m * N + n] = from_float<T>(silu_mul(__uint_as_float(v[i]) + bias, swap[i * 64 + r]));
+                        }
+                    }
+                    named_barrier_sync(1, kEpiThreads);
+                } else if (ok) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const int m = c * 32 + i;
+                        if (live && m < M) out[(size_t)m * N + n] = from_float<T>(__uint_as_float(v[i]) + bias);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.tmem_empty[buf]);
+        }
+    }
+
+    // ---------------------------------------------------------------------- teardown
+    if (*bars.abort_flag != 0) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) { }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp_id == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 256);
+    }
+}
+
+template <typename T, int G, bool GATED>
+int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
+                  const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
+    static bool ready[64] = {};
+    auto kern = int4_tokens_kernel<T, G, GATED>;
+    constexpr int kMaxSmem = 227 * 1024, kFixed = kRing * 2 * kSlab + kSwapBytes + 512;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!ready[dev & 63]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess)
+            return kLaunchFailed;
+        ready[dev & 63] = true;
+    }
+    const int cols = (M + 15) / 16 * 16;
+    const int ring_x = std::min((kMaxSmem - kFixed) / (2 * cols * 128), kMaxRingX);
+    // rows of a CTA: as many as its lanes hold, or fewer so that every SM makes the same number
+    const int most = GATED ? 64 : 128, sms = sm_count();
+    const int waves = (int)(((long long)N + (long long)most * sms - 1) / ((long long)most * sms));
+    const int rows = (int)(((long long)N + (long long)waves * sms - 1) / ((long long)waves * sms));
+    const int tiles = (int)(((long long)N + rows - 1) / rows);
+    CUtensorMap tm_x;
+    if (!encode_sw128(&tm_x, type16(std::is_same<T, __nv_bfloat16>::value), 2, x, K, M, cols)) return kLaunchFailed;
+    int* status = status_word();
+    if (status == nullptr) return kLaunchFailed;
+    kern<<<std::min(tiles, sms), kThreads, kFixed + ring_x * 2 * cols * 128, stream>>>(
+        tm_x, w0, w1, s0, s1, static_cast<const T*>(b0), static_cast<const T*>(b1), static_cast<T*>(out), M, N, K, rows, cols,
+        ring_x, status);
+    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+}
+
 template <typename T, int G, bool GATED, int BN>
 int launch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
            const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
@@ -426,6 +752,9 @@ template <typename T, int G>
 int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
              const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
     const bool gated = w1 != nullptr;
+    if (M <= kTokensMax)
+        return gated ? launch_tokens<T, G, true>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                     : launch_tokens<T, G, false>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     // 128 weight rows a tile take 0.6 of the time of 256 (tensor instructions of 128 columns run at their floor of 86
     // clocks): where even those leave pairs without a tile
     const long long wide = ((long long)M + 255) / 256 * (((long long)N * (gated ? 2 : 1) + 255) / 256);

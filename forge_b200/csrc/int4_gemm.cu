@@ -411,6 +411,9 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 // a multiple of 16), so the tensor instructions shrink with the batch, and what bounds the call is how fast weights become
 // operands. One CTA per tile of `rows` rows (gated: of each matrix, Wg in lanes 0-63 and Wu in lanes 64-127), chosen so
 // that all SMs have the same number; rows beyond it are stale shared memory in accumulator lanes of their own, not stored.
+// A tensor instruction of so few columns takes 75 clocks however few there are, so a tile costs 600 clocks a block of 128
+// inputs; where 128-row tiles leave SMs free, a cluster of CTAs divides a tile's inputs, and sums its parts through
+// distributed shared memory, in rank order (4096 x 14336, 64 tokens: 61 us without).
 // Weights and activations have rings of their own: a weight stage (32 KB) is made within half a microsecond of being
 // free, while a copy of activations takes a whole one (one ring of three for both, on CTA pairs: 33 us for every batch).
 struct TokenBars {
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
                    const __half* __restrict__ s0, const __half* __restrict__ s1, const T* __restrict__ b0,
                    const T* __restrict__ b1, T* __restrict__ out, int M, int N, int K, int rows, int cols, int ring_x,
-                   int* __restrict__ status) {
+                   int split, int* __restrict__ status) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     constexpr int PER = 128 / G;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -467,7 +470,12 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         return;
     }
     const int num_tiles = (N + rows - 1) / rows;
-    const int blocks = (K + 127) / 128;
+    // a cluster has one tile, a CTA without one takes every gridDim.x-th
+    const int rank = split > 1 ? (int)(blockIdx.x % split) : 0;
+    const int first_tile = blockIdx.x / split, tile_step = gridDim.x / split;
+    const int all_blocks = (K + 127) / 128;
+    const int blk0 = (int)((long long)all_blocks * rank / split);                    // of this CTA
+    const int blocks = (int)((long long)all_blocks * (rank + 1) / split) - blk0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRing; s++) {
@@ -500,7 +508,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+            for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
                 for (int blk = 0; blk < blocks; blk++) {
                     if (!mbar_wait(&bars.empty_x[stage], phase ^ 1, bars.abort_flag)) {
                         atomicExch(status, 851);
@@ -509,8 +517,8 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     }
                     uint8_t* dst = smem_x + stage * 2 * slab_x;
                     mbar_expect_tx(&bars.full_x[stage], 2 * slab_x);
-                    tma_load_2d(dst, &tm_x, &bars.full_x[stage], blk * 128, 0);
-                    tma_load_2d(dst + slab_x, &tm_x, &bars.full_x[stage], blk * 128 + 64, 0);
+                    tma_load_2d(dst, &tm_x, &bars.full_x[stage], (blk0 + blk) * 128, 0);
+                    tma_load_2d(dst + slab_x, &tm_x, &bars.full_x[stage], (blk0 + blk) * 128 + 64, 0);
                     if (++stage == ring_x) {
                         stage = 0;
                         phase ^= 1;
@@ -525,7 +533,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             int stage = 0, stage_x = 0, local = 0;
             uint32_t phase = 0, phase_x = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, local++) {
+            for (int t = first_tile; t < num_tiles && ok; t += tile_step, local++) {
                 const int buf = local & 1;
                 if (!mbar_wait(&bars.tmem_empty[buf], ((local >> 1) & 1) ^ 1, bars.abort_flag)) {
                     atomicExch(status, 852);
@@ -576,14 +584,14 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         int blk = group;
         // i-th row of a lane: i * 32 + local_row (gated: rows 0-31 and 32-63 of Wg, then of Wu)
         auto used = [&](int i) { return (GATED ? i % 2 : i) * 8 * kGroupWarps < rows; };
-        for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
             const uint8_t* wp[ROWS];
             const unsigned short* sp[ROWS];
 #pragma unroll
             for (int i = 0; i < ROWS; i++) {
                 const bool second = GATED && i >= ROWS / 2;
                 const int row = min(t * rows + (GATED ? i % 2 : i) * 8 * kGroupWarps + local_row, N - 1);
-                wp[i] = (second ? w1 : w0) + (size_t)row * ((size_t)blocks * 64) + t4 * 16;
+                wp[i] = (second ? w1 : w0) + (size_t)row * ((size_t)all_blocks * 64) + (size_t)blk0 * 64 + t4 * 16;
                 sp[i] = reinterpret_cast<const unsigned short*>(second ? s1 : s0) + row;
             }
             uint4 next[2][ROWS];   // of the stage's next block and the one behind it
@@ -594,7 +602,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     if (used(i)) {
                         v[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
 #pragma unroll
-                        for (int k = 0; k < PER; k++) sc[i][k] = __ldg(sp[i] + (size_t)min(b * PER + k, groups - 1) * N);
+                        for (int k = 0; k < PER; k++) sc[i][k] = __ldg(sp[i] + (size_t)min((blk0 + b) * PER + k, groups - 1) * N);
                     }
             };
             auto make = [&](uint4 (&v)[ROWS], unsigned short (&sc)[ROWS][PER]) {
@@ -637,7 +645,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         float* swap = reinterpret_cast<float*>(smem_swap);
         int local = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, local++) {
+        for (int t = first_tile; t < num_tiles; t += tile_step, local++) {
             const int buf = local & 1;
             const int r = GATED ? (q % 2) * 32 + lane : q * 32 + lane;
             const int n = t * rows + r;
@@ -656,6 +664,13 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                 if (ok) {
                     tmem_ld_32x32b_x32(taddr + c * 32, v);
                     tmem_ld_wait();
+                }
+                if (split > 1) {   // this CTA's part, where the weights were
+                    float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (c * 32 + i < cols) part[(c * 32 + i) * 128] = __uint_as_float(v[i]);
+                    continue;
                 }
                 if constexpr (GATED) {
                     if (q >= 2 && ok) {
@@ -697,6 +712,35 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         tc_fence_after();
         tmem_dealloc(tmem_base, 256);
     }
+    if (split > 1) {
+        cluster_sync_all();   // all parts are there
+        if (*bars.abort_flag == 0) {
+            const uint32_t part = smem_u32(smem);
+            auto sum = [&](int m, int r) {
+                float v = 0.f;
+                for (int c = 0; c < split; c++) {
+                    float p;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                 : "=f"(p)
+                                 : "r"(mapa_shared(part + (m * 128 + r) * 4, c))
+                                 : "memory");
+                    v += p;
+                }
+                return v;
+            };
+            // every split-th token is this CTA's
+            constexpr int LANES = GATED ? 64 : 128;
+            for (int i = threadIdx.x; i < (M - rank + split - 1) / split * LANES; i += kThreads) {
+                const int m = rank + i / LANES * split, r = i % LANES, n = first_tile * rows + r;
+                if (r < rows && n < N) {
+                    float v = sum(m, r) + (b0 != nullptr ? to_float(b0[n]) : 0.f);
+                    if constexpr (GATED) v = silu_mul(v, sum(m, 64 + r) + (b1 != nullptr ? to_float(b1[n]) : 0.f));
+                    out[(size_t)m * N + n] = from_float<T>(v);
+                }
+            }
+        }
+        cluster_sync_all();   // nobody reads this CTA's memory any more
+    }
 }
 
 template <typename T, int G, bool GATED>
@@ -714,19 +758,34 @@ int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __h
     }
     const int cols = (M + 15) / 16 * 16;
     const int ring_x = std::min((kMaxSmem - kFixed) / (2 * cols * 128), kMaxRingX);
-    // rows of a CTA: as many as its lanes hold, or fewer so that every SM makes the same number
-    const int most = GATED ? 64 : 128, sms = sm_count();
-    const int waves = (int)(((long long)N + (long long)most * sms - 1) / ((long long)most * sms));
-    const int rows = (int)(((long long)N + (long long)waves * sms - 1) / ((long long)waves * sms));
+    const int most = GATED ? 64 : 128, sms = sm_count(), blocks = (K + 127) / 128;
+    const long long full = ((long long)N + most - 1) / most;   // tiles of as many rows as the lanes hold
+    int split = 1;
+    while (split < 8 && full * split * 2 <= sms && blocks >= 4 * split) split *= 2;
+    // without a split, so many rows that every SM has the same number
+    const int waves = (int)((full + sms - 1) / sms);
+    const int rows = split > 1 ? most : (int)(((long long)N + (long long)waves * sms - 1) / ((long long)waves * sms));
     const int tiles = (int)(((long long)N + rows - 1) / rows);
     CUtensorMap tm_x;
     if (!encode_sw128(&tm_x, type16(std::is_same<T, __nv_bfloat16>::value), 2, x, K, M, cols)) return kLaunchFailed;
     int* status = status_word();
     if (status == nullptr) return kLaunchFailed;
-    kern<<<std::min(tiles, sms), kThreads, kFixed + ring_x * 2 * cols * 128, stream>>>(
-        tm_x, w0, w1, s0, s1, static_cast<const T*>(b0), static_cast<const T*>(b1), static_cast<T*>(out), M, N, K, rows, cols,
-        ring_x, status);
-    return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(split > 1 ? tiles * split : std::min(tiles, sms), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kFixed + ring_x * 2 * cols * 128;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, tm_x, w0, w1, s0, s1, static_cast<const T*>(b0), static_cast<const T*>(b1),
+                              static_cast<T*>(out), M, N, K, rows, cols, ring_x, split, status) == cudaSuccess
+               ? kOk
+               : kLaunchFailed;
 }
 
 template <typename T, int G, bool GATED, int BN>

@@ -107,10 +107,10 @@ def test_int4_linear(M, K, N, group, dtype):
 
 
 def linear_bound(x, w, s, b, group):
-    """Up to 8 tokens as R.int4_sizes says; above a weight is rounded once to the activations' type."""
+    """Up to 16 tokens as R.int4_sizes says; above a weight is rounded once to the activations' type."""
     K = x.shape[1]
     weight = R.unpack_int4(w, s, K, group)
-    if x.shape[0] <= 8:
+    if x.shape[0] <= 16:
         return R.linear(x, weight, b, R.int4_sizes(s, K, group, x.dtype), group)
     y, err = R.linear(x, weight, b)
     return y, err + x.double().abs() @ R.half_step(weight, x.dtype).t()

@@ -6,15 +6,17 @@
 //
 // The skeleton of the other pair kernels (256 tokens x BN weight rows per pair), with the weight's TMA producer replaced by
 // twelve warps per CTA that read packed weights from L2, multiply the integers by their scales and write 16-bit numbers
-// in the swizzled layout that the tensor cores read; nothing of the unpacked weight ever reaches memory. Gated, CTA 0
-// makes rows of Wg and CTA 1 the same rows of Wu. A stage is a whole block of 128 inputs (three of 64 KB). Making one takes
-// longer than the tensor cores need for it, so each stage has four warps of its own, three blocks being made at a time; the
-// warps signal a barrier of their own CTA only, and one thread passes CTA 1's on to the leader (with eight warps on each
-// 64-deep slab in turn and arrivals across the cluster, 2048 x 4096 x 11008 took 308 us).
+// in the swizzled layout that the tensor cores read; nothing of the unpacked weight ever reaches memory. A stage is a
+// whole block of 128 inputs (three of 64 KB). Making one takes longer than the tensor cores need for it, so each stage has
+// four warps of its own, three blocks being made at a time; the warps signal a barrier of their own CTA only, and one
+// thread passes CTA 1's on to the leader (with eight warps on each 64-deep slab in turn and arrivals across the cluster,
+// 2048 x 4096 x 11008 took 308 us; 142 us like this, 1300 TFLOP/s).
 //
-// A weight is rounded once, to the activations' type, as s q: exactly the product of the two, rounded (bf16: s is split
-// into two bf16 numbers whose products with q are exact, so that one fused multiply-add rounds their sum). That is one
-// rounding more than the few-token kernel has; accumulators are fp32.
+// s q has more bits than a 16-bit number. Plain calls round it once, which with the rounding of the output makes 1.4 times
+// (fp16: 1.25 times) the error of the latter. Behind the gate two such products would meet and make it 1.7 times, so
+// gated calls take both parts: CTA 0 makes the rounded weights and CTA 1 what the rounding left, which is exact, for the
+// same 64 rows of both matrices; their products lie in neighbouring accumulator columns and are added in the epilogue.
+// That is twice the tensor work (333 tokens, 4096 x 14336: TIME1 instead of 114 us) and no error beyond fp32 sums.
 #include <algorithm>
 #include <type_traits>
 
@@ -55,50 +57,67 @@ __device__ __forceinline__ RingBars carve_ring(uint8_t* p) {
 }
 constexpr int kThreads = 32 * (2 + kEpiWarps + kWeightWarps);   // TMA warp, MMA warp, epilogue, weights
 
-// Word of 8 four-bit weights times its scale -> 8 numbers of type T in order. A nibble in the low mantissa bits of 1024
+// Word of 8 four-bit weights -> the integers q as 8 numbers of type T in order. A nibble in the low mantissa bits of 1024
 // (fp16) or 128 (bf16) is that number plus the nibble, exactly; subtracting the offset + 8 leaves q, exactly.
+__device__ __forceinline__ void unpack_q(uint32_t w, __half2 (&q)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t v = w >> (8 * i);
+        const uint32_t lo = and_or(v, 0x000F000Fu, 0x64006400u), hi = and_or(v, 0x00F000F0u, 0x64006400u);
+        q[2 * i] = __hsub2(reinterpret_cast<const __half2&>(lo), __half2half2(__ushort_as_half(0x6408)));
+        q[2 * i + 1] = __hfma2(reinterpret_cast<const __half2&>(hi), __half2half2(__ushort_as_half(0x2C00)),
+                               __half2half2(__ushort_as_half(0xD480)));   // / 16 - 72
+    }
+}
+__device__ __forceinline__ void unpack_q(uint32_t w, __nv_bfloat162 (&q)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+        q[i] = __hsub2(reinterpret_cast<const __nv_bfloat162&>(b), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
+    }
+}
+template <typename V>
+__device__ __forceinline__ uint4 bits4(const V (&v)[4]) {
+    return make_uint4(reinterpret_cast<const uint32_t&>(v[0]), reinterpret_cast<const uint32_t&>(v[1]),
+                      reinterpret_cast<const uint32_t&>(v[2]), reinterpret_cast<const uint32_t&>(v[3]));
+}
+
+// A word's weights s q rounded to T, or (`rest`) what that rounding left, exactly.
 template <typename T>
 struct Scaled;
 template <>
 struct Scaled<__half> {
     __half2 s;
     __device__ __forceinline__ explicit Scaled(unsigned short bits) : s(__half2half2(__ushort_as_half(bits))) {}
-    __device__ __forceinline__ uint4 operator()(uint32_t w) const {
-        uint32_t f[4];
+    __device__ __forceinline__ uint4 operator()(uint32_t w, bool rest) const {
+        __half2 q[4];
+        unpack_q(w, q);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t v = w >> (8 * i);
-            const uint32_t lo = and_or(v, 0x000F000Fu, 0x64006400u), hi = and_or(v, 0x00F000F0u, 0x64006400u);
-            const __half2 a = __hsub2(reinterpret_cast<const __half2&>(lo), __half2half2(__ushort_as_half(0x6408)));
-            const __half2 b = __hfma2(reinterpret_cast<const __half2&>(hi), __half2half2(__ushort_as_half(0x2C00)),
-                                      __half2half2(__ushort_as_half(0xD480)));   // / 16 - 72
-            const __half2 x = __hmul2(a, s), y = __hmul2(b, s);
-            f[2 * i] = reinterpret_cast<const uint32_t&>(x);
-            f[2 * i + 1] = reinterpret_cast<const uint32_t&>(y);
+        for (int i = 0; i < 4; i++) {
+            const __half2 v = __hmul2(q[i], s);
+            q[i] = rest ? __hfma2(q[i], s, __hneg2(v)) : v;   // a multiple of 2^-24 as s is, so never out of range below
         }
-        return make_uint4(f[0], f[1], f[2], f[3]);
+        return bits4(q);
     }
 };
 template <>
 struct Scaled<__nv_bfloat16> {
-    __nv_bfloat162 hi, lo;
+    __nv_bfloat162 hi, lo;   // s = hi + lo; their products with q are exact
     __device__ __forceinline__ explicit Scaled(unsigned short bits) {
         const float s = __half2float(__ushort_as_half(bits));
         const __nv_bfloat16 h = __float2bfloat16_rn(s);
         hi = __bfloat162bfloat162(h);
         lo = __bfloat162bfloat162(__float2bfloat16_rn(s - __bfloat162float(h)));
     }
-    __device__ __forceinline__ uint4 operator()(uint32_t w) const {
-        uint32_t f[4];
+    __device__ __forceinline__ uint4 operator()(uint32_t w, bool rest) const {
+        __nv_bfloat162 q[4];
+        unpack_q(w, q);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
-            const __nv_bfloat162 q =
-                __hsub2(reinterpret_cast<const __nv_bfloat162&>(b), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
-            const __nv_bfloat162 v = __hfma2(q, hi, __hmul2(q, lo));
-            f[i] = reinterpret_cast<const uint32_t&>(v);
+            const __nv_bfloat162 small = __hmul2(q[i], lo), v = __hfma2(q[i], hi, small);
+            q[i] = rest ? __hadd2(__hfma2(q[i], hi, __hneg2(v)), small) : v;
         }
-        return make_uint4(f[0], f[1], f[2], f[3]);
+        return bits4(q);
     }
 };
 
@@ -119,7 +138,7 @@ __device__ __forceinline__ void relay(const RingBars& bars, long long turns, int
     }
 }
 
-// BN: weight rows per tile (256 or 128), of both matrices when GATED.
+// BN: rows of the pair's weight operand (256 or 128); GATED 256: 64 rows of each matrix, rounded and rest.
 template <typename T, int G, bool GATED, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
 int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out,
@@ -127,7 +146,8 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                  const __half* __restrict__ s1, const T* __restrict__ b0, const T* __restrict__ b1, T* __restrict__ out,
                  int M, int N, int K, int tma_out, int* __restrict__ status) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    constexpr int TILE_N = GATED ? BN / 2 : BN;   // output columns
+    static_assert(!GATED || BN == 256, "the gated tile");
+    constexpr int TILE_N = GATED ? BN / 4 : BN;   // output columns
     constexpr int HALF = BN / 2;                  // weight rows that a CTA makes
     constexpr int PER = 128 / G;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -250,8 +270,6 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         const int row8 = (lane >> 3) | ((lane >> 2) & 1) << 2;
         const int group = (warp_id - 2 - kEpiWarps) / kGroupWarps;
         const int local_row = (warp_id - 2 - kEpiWarps) % kGroupWarps * 8 + row8;
-        const uint8_t* w = GATED && rank == 1 ? w1 : w0;
-        const unsigned short* s = reinterpret_cast<const unsigned short*>(GATED && rank == 1 ? s1 : s0);
         const int groups = (K + G - 1) / G;
         // Every third block of those that the CTA goes through, always into the same stage: a barrier's parity tells a lap
         // from its neighbours only, so whoever waits on it has to see every lap.
@@ -262,11 +280,14 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
         for (int t = pair_id; t < num_tiles && ok; t += num_pairs) {
             const Tile tc = tile_of(t, a_blocks, b_blocks);
             const uint8_t* wp[ROWS];
-            int row[ROWS];
+            const unsigned short* sp[ROWS];
 #pragma unroll
             for (int i = 0; i < ROWS; i++) {
-                row[i] = min(tc.b_blk * TILE_N + (GATED ? 0 : (int)rank * HALF) + local_row + 8 * kGroupWarps * i, N - 1);
-                wp[i] = w + (size_t)row[i] * ((size_t)blocks * 64) + t4 * 16;
+                const bool second = GATED && i >= ROWS / 2;   // gated: 64 rows of Wg, then the same of Wu
+                const int r = local_row + 8 * kGroupWarps * (GATED ? i % (ROWS / 2) : i);
+                const int row = min(tc.b_blk * TILE_N + (GATED ? 0 : (int)rank * HALF) + r, N - 1);
+                wp[i] = (second ? w1 : w0) + (size_t)row * ((size_t)blocks * 64) + t4 * 16;
+                sp[i] = reinterpret_cast<const unsigned short*>(second ? s1 : s0) + row;
             }
             uint4 next[ROWS];
             unsigned short next_s[ROWS][PER];
@@ -275,7 +296,7 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                 for (int i = 0; i < ROWS; i++) {
                     next[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
 #pragma unroll
-                    for (int k = 0; k < PER; k++) next_s[i][k] = __ldg(s + (size_t)min(b * PER + k, groups - 1) * N + row[i]);
+                    for (int k = 0; k < PER; k++) next_s[i][k] = __ldg(sp[i] + (size_t)min(b * PER + k, groups - 1) * N);
                 }
             };
             if (blk < blocks) load(blk);
@@ -303,7 +324,7 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
                     for (int j = 0; j < 4; j++)
                         *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (8 * kGroupWarps * 128) +
                                                   (((4 * (j % 2) + t4) ^ row8) << 4)) =
-                            Scaled<T>(cur_s[i][j * 32 / G])(word[j]);
+                            Scaled<T>(cur_s[i][j * 32 / G])(word[j], GATED && rank == 1);
                 }
                 fence_proxy_async_smem();   // the tensor cores read through the async proxy
                 __syncwarp();
@@ -325,7 +346,7 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             const int row0 = tc.a_blk * 256 + (int)rank * 128 + q * 32;
             const int n0 = tc.b_blk * TILE_N;
             float* bias = smem_bias + buf * 256;   // TILE_N of b0; gated: then TILE_N of b1
-            for (int i = epi_tid; i < BN; i += kEpiThreads) {
+            for (int i = epi_tid; i < (GATED ? 2 : 1) * TILE_N; i += kEpiThreads) {
                 const int n = n0 + i % TILE_N;
                 const T* b = i < TILE_N ? b0 : b1;
                 bias[i] = b != nullptr && n < N ? to_float(b[n]) : 0.f;
@@ -342,21 +363,33 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
             for (int c = 0; c < TILE_N / 64; c++) {
                 uint32_t packed[32];
 #pragma unroll
-                for (int hh = 0; hh < 2; hh++) {
-                    const int col = c * 64 + hh * 32;
-                    uint32_t va[32], vb[32];
-                    tmem_ld_32x32b_x32(taddr + col, va);
-                    if (GATED) tmem_ld_32x32b_x32(taddr + TILE_N + col, vb);
-                    tmem_ld_wait();
+                for (int hh = 0; hh < 4; hh++) {
+                    const int col = c * 64 + hh * 16;
+                    uint32_t va[16], vb[16];
+                    tmem_ld_32x32b_x16(taddr + col, va);
+                    if (GATED) {   // gate, up, and the products of what the rounding left
+                        uint32_t ra[16], rb[16];
+                        tmem_ld_32x32b_x16(taddr + TILE_N + col, vb);
+                        tmem_ld_32x32b_x16(taddr + 2 * TILE_N + col, ra);
+                        tmem_ld_32x32b_x16(taddr + 3 * TILE_N + col, rb);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
+                        for (int i = 0; i < 16; i++) {
+                            va[i] = __float_as_uint(__uint_as_float(va[i]) + __uint_as_float(ra[i]));
+                            vb[i] = __float_as_uint(__uint_as_float(vb[i]) + __uint_as_float(rb[i]));
+                        }
+                    } else {
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
                         float o[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             o[e] = __uint_as_float(va[2 * i + e]) + bias[col + 2 * i + e];
                             if (GATED) o[e] = silu_mul(o[e], __uint_as_float(vb[2 * i + e]) + bias[TILE_N + col + 2 * i + e]);
                         }
-                        packed[hh * 16 + i] = pack2<T>(o[0], o[1]);
+                        packed[hh * 8 + i] = pack2<T>(o[0], o[1]);
                     }
                 }
                 if (row0 >= M || n0 + c * 64 >= N) continue;   // nothing to store; a box must not start outside
@@ -408,22 +441,28 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 }
 
 // Up to 128 tokens: the operands change places. Weight rows are the lanes, tokens the columns, as many as there are (`cols`,
-// a multiple of 16), so the tensor instructions shrink with the batch, and what bounds the call is how fast weights become
+// a multiple of 32), so the tensor instructions shrink with the batch, and what bounds the call is how fast weights become
 // operands. One CTA per tile of `rows` rows (gated: of each matrix, Wg in lanes 0-63 and Wu in lanes 64-127), chosen so
 // that all SMs have the same number; rows beyond it are stale shared memory in accumulator lanes of their own, not stored.
 // A tensor instruction of so few columns takes 75 clocks however few there are, so a tile costs 600 clocks a block of 128
 // inputs; where 128-row tiles leave SMs free, a cluster of CTAs divides a tile's inputs, and sums its parts through
-// distributed shared memory, in rank order (4096 x 14336, 64 tokens: 61 us without).
-// Weights and activations have rings of their own: a weight stage (32 KB) is made within half a microsecond of being
-// free, while a copy of activations takes a whole one (one ring of three for both, on CTA pairs: 33 us for every batch).
+// distributed shared memory, in rank order (4096 x 14336, 64 tokens: 61 us without, 30 with).
+//
+// With so few columns there is time to keep the sums exact: the operand holds the integers, every group of inputs has
+// accumulator columns of its own (a ring of four), and eight warps multiply them by the scale of their lane's row and
+// add them up in registers, in fp32. Nothing is rounded before the result.
 struct TokenBars {
     uint64_t *full_w, *empty_w;   // [kRing]: the stage's weight warps; committed by the MMA thread
     uint64_t *full_x, *empty_x;   // [kMaxRingX]
-    uint64_t *tmem_full, *tmem_empty;
+    uint64_t *tmem_full, *tmem_empty;   // [kAccs]
     uint32_t* tmem_slot;
     volatile int* abort_flag;
 };
 constexpr int kMaxRingX = 8;
+constexpr int kAccs = 4;                  // accumulators of up to 128 columns
+constexpr int kSumWarps = 8;              // two for each quarter of the lanes, half of the columns each
+constexpr int kTokenGroupWarps = 2;       // that make a stage's weights
+constexpr int kTokenThreads = 32 * (2 + kSumWarps + kRing * kTokenGroupWarps);
 constexpr int kSwapBytes = 32 * 64 * 4;   // gated: the up products of 32 tokens x 64 rows
 __device__ __forceinline__ TokenBars carve_tokens(uint8_t* p) {
     TokenBars b;
@@ -432,8 +471,8 @@ __device__ __forceinline__ TokenBars carve_tokens(uint8_t* p) {
     b.full_x = b.empty_w + kRing;
     b.empty_x = b.full_x + kMaxRingX;
     b.tmem_full = b.empty_x + kMaxRingX;
-    b.tmem_empty = b.tmem_full + 2;
-    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + 2);
+    b.tmem_empty = b.tmem_full + kAccs;
+    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + kAccs);
     b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
     return b;
 }
@@ -450,7 +489,7 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uin
 }
 
 template <typename T, int G, bool GATED>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kTokenThreads, 1)
 int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
                    const __half* __restrict__ s0, const __half* __restrict__ s1, const T* __restrict__ b0,
                    const T* __restrict__ b1, T* __restrict__ out, int M, int N, int K, int rows, int cols, int ring_x,
@@ -479,22 +518,22 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kRing; s++) {
-            mbar_init(&bars.full_w[s], kGroupWarps);
+            mbar_init(&bars.full_w[s], kTokenGroupWarps);
             mbar_init(&bars.empty_w[s], 1);
         }
         for (int s = 0; s < ring_x; s++) {
             mbar_init(&bars.full_x[s], 1);
             mbar_init(&bars.empty_x[s], 1);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < kAccs; i++) {
             mbar_init(&bars.tmem_full[i], 1);
-            mbar_init(&bars.tmem_empty[i], kEpiWarps);
+            mbar_init(&bars.tmem_empty[i], kSumWarps);
         }
         *bars.abort_flag = 0;
         fence_mbar_init();
     }
     if (warp_id == 1) {
-        tmem_alloc(bars.tmem_slot, 256);
+        tmem_alloc(bars.tmem_slot, 128 * kAccs);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -530,19 +569,11 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         // ------------------------------------------------------------------ MMA issuer
         if (lane == 0) {
             const uint32_t idesc = idesc_f16(128, cols, BF16, false, false);
-            int stage = 0, stage_x = 0, local = 0;
-            uint32_t phase = 0, phase_x = 0;
+            int stage = 0, stage_x = 0, acc = 0;
+            uint32_t phase = 0, phase_x = 0, phase_acc = 0;
             bool ok = true;
-            for (int t = first_tile; t < num_tiles && ok; t += tile_step, local++) {
-                const int buf = local & 1;
-                if (!mbar_wait(&bars.tmem_empty[buf], ((local >> 1) & 1) ^ 1, bars.abort_flag)) {
-                    atomicExch(status, 852);
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t acc = tmem_base + buf * 128;
-                for (int blk = 0; blk < blocks; blk++) {
+            for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+                for (int blk = 0; blk < blocks && ok; blk++) {
                     if (!mbar_wait(&bars.full_x[stage_x], phase_x, bars.abort_flag) ||
                         !mbar_wait(&bars.full_w[stage], phase, bars.abort_flag)) {
                         atomicExch(status, 853);
@@ -553,9 +584,25 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     const uint64_t da = make_desc_sw128(smem_u32(smem + stage * 2 * kSlab));
                     const uint64_t db = make_desc_sw128(smem_u32(smem_x + stage_x * 2 * slab_x));
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        umma_f16(acc, da + (k / 4) * (kSlab >> 4) + 2 * (k % 4), db + (k / 4) * (slab_x >> 4) + 2 * (k % 4),
-                                 idesc, (blk | k) != 0 ? 1u : 0u);
+                    for (int k = 0; k < 8; k++) {
+                        if (k % (G / 16) == 0) {
+                            if (!mbar_wait(&bars.tmem_empty[acc], phase_acc ^ 1, bars.abort_flag)) {
+                                atomicExch(status, 852);
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                        }
+                        umma_f16(tmem_base + acc * 128, da + (k / 4) * (kSlab >> 4) + 2 * (k % 4),
+                                 db + (k / 4) * (slab_x >> 4) + 2 * (k % 4), idesc, k % (G / 16) != 0 ? 1u : 0u);
+                        if (k % (G / 16) == G / 16 - 1) {
+                            tc_commit(&bars.tmem_full[acc]);
+                            if (++acc == kAccs) {
+                                acc = 0;
+                                phase_acc ^= 1;
+                            }
+                        }
+                    }
                     tc_commit(&bars.empty_w[stage]);
                     tc_commit(&bars.empty_x[stage_x]);
                     if (++stage == kRing) {
@@ -567,137 +614,172 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                         phase_x ^= 1;
                     }
                 }
-                if (ok) tc_commit(&bars.tmem_full[buf]);
             }
         }
-    } else if (warp_id >= 2 + kEpiWarps) {
-        // ------------------------------------------------------------------ weights, as in int4_pair_kernel
-        constexpr int ROWS = 4;   // of a lane; the last ones only where a CTA has so many
+    } else if (warp_id >= 2 + kSumWarps) {
+        // ------------------------------------------------------------------ weights, as in int4_pair_kernel, unscaled
+        constexpr int ROWS = 128 / (8 * kTokenGroupWarps);   // of a lane; the last ones only where a CTA has so many
+        constexpr int STEP = 8 * kTokenGroupWarps;
         const int t4 = lane & 3;
         const int row8 = (lane >> 3) | ((lane >> 2) & 1) << 2;
-        const int group = (warp_id - 2 - kEpiWarps) / kGroupWarps;
-        const int local_row = (warp_id - 2 - kEpiWarps) % kGroupWarps * 8 + row8;
-        const int groups = (K + G - 1) / G;
-        const int stage = group;
+        const int stage = (warp_id - 2 - kSumWarps) / kTokenGroupWarps;
+        const int local_row = (warp_id - 2 - kSumWarps) % kTokenGroupWarps * 8 + row8;
         uint32_t phase = 0;
         bool ok = true;
-        int blk = group;
-        // i-th row of a lane: i * 32 + local_row (gated: rows 0-31 and 32-63 of Wg, then of Wu)
-        auto used = [&](int i) { return (GATED ? i % 2 : i) * 8 * kGroupWarps < rows; };
+        int blk = stage;   // of its tile
+        // i-th row of a lane: i * STEP + local_row (gated: 64 rows of Wg, then of Wu)
+        auto used = [&](int i) { return (GATED ? i % (ROWS / 2) : i) * STEP < rows; };
         for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+            auto row_of = [&](int i) {
+                const int row = min(t * rows + (GATED ? i % (ROWS / 2) : i) * STEP + local_row, N - 1);
+                return (GATED && i >= ROWS / 2 ? w1 : w0) + (size_t)row * ((size_t)all_blocks * 64) + (size_t)blk0 * 64 + t4 * 16;
+            };
             const uint8_t* wp[ROWS];
-            const unsigned short* sp[ROWS];
 #pragma unroll
-            for (int i = 0; i < ROWS; i++) {
-                const bool second = GATED && i >= ROWS / 2;
-                const int row = min(t * rows + (GATED ? i % 2 : i) * 8 * kGroupWarps + local_row, N - 1);
-                wp[i] = (second ? w1 : w0) + (size_t)row * ((size_t)all_blocks * 64) + (size_t)blk0 * 64 + t4 * 16;
-                sp[i] = reinterpret_cast<const unsigned short*>(second ? s1 : s0) + row;
-            }
-            uint4 next[2][ROWS];   // of the stage's next block and the one behind it
-            unsigned short next_s[2][ROWS][PER];
-            auto load = [&](int b, uint4 (&v)[ROWS], unsigned short (&sc)[ROWS][PER]) {
+            for (int i = 0; i < ROWS; i++) wp[i] = row_of(i);
+            uint4 next[ROWS];
+            auto load = [&](int b) {
 #pragma unroll
                 for (int i = 0; i < ROWS; i++)
-                    if (used(i)) {
-                        v[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
-#pragma unroll
-                        for (int k = 0; k < PER; k++) sc[i][k] = __ldg(sp[i] + (size_t)min((blk0 + b) * PER + k, groups - 1) * N);
-                    }
+                    if (used(i)) next[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
             };
-            auto make = [&](uint4 (&v)[ROWS], unsigned short (&sc)[ROWS][PER]) {
+            load(min(blk, blocks - 1));
+            for (; blk < blocks; blk += kRing) {
+                // All of the next block's loads behind all uses of this one's: a load between two uses makes the second
+                // wait for it (870 clocks a row).
+                uint4 cur[ROWS];
+#pragma unroll
+                for (int i = 0; i < ROWS; i++)
+                    if (used(i)) cur[i] = next[i];
+                load(min(blk + kRing, blocks - 1));
                 ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty_w[stage], phase ^ 1, bars.abort_flag));
                 if (!ok) {
                     if (lane == 0) atomicExch(status, 854);
-                    return;
+                    break;
                 }
                 phase ^= 1;
                 uint8_t* dst = smem + stage * 2 * kSlab + local_row * 128;
 #pragma unroll
                 for (int i = 0; i < ROWS; i++)
                     if (used(i)) {
-                        const uint32_t word[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                        const uint32_t word[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (8 * kGroupWarps * 128) +
-                                                      (((4 * (j % 2) + t4) ^ row8) << 4)) = Scaled<T>(sc[i][j * 32 / G])(word[j]);
+                        for (int j = 0; j < 4; j++) {
+                            typename std::conditional<BF16, __nv_bfloat162, __half2>::type q[4];
+                            unpack_q(word[j], q);
+                            *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (STEP * 128) +
+                                                      (((4 * (j % 2) + t4) ^ row8) << 4)) = bits4(q);
+                        }
                     }
                 fence_proxy_async_smem();   // the tensor cores read through the async proxy
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.full_w[stage]);
-            };
-            load(min(blk, blocks - 1), next[0], next_s[0]);
-            load(min(blk + kRing, blocks - 1), next[1], next_s[1]);
-            while (blk < blocks && ok) {
-                make(next[0], next_s[0]);
-                load(min(blk + 2 * kRing, blocks - 1), next[0], next_s[0]);
-                blk += kRing;
-                if (blk >= blocks || !ok) break;
-                make(next[1], next_s[1]);
-                load(min(blk + 2 * kRing, blocks - 1), next[1], next_s[1]);
-                blk += kRing;
             }
             blk -= blocks;
         }
     } else {
-        // ------------------------------------------------------------------ epilogue: a lane has a row's products with all tokens
-        const int q = warp_id & 3;
+        // ------------------------------------------------------------------ sums: a lane has a row's products with half of the tokens
+        const int q = warp_id & 3, half = (warp_id - 2) / 4;
+        const int width = cols / 2, col0 = half * width;   // a multiple of 16, at most 64
         float* swap = reinterpret_cast<float*>(smem_swap);
-        int local = 0;
+        int acc = 0;
+        uint32_t phase_acc = 0;
         bool ok = true;
-        for (int t = first_tile; t < num_tiles; t += tile_step, local++) {
-            const int buf = local & 1;
+        for (int t = first_tile; t < num_tiles; t += tile_step) {
             const int r = GATED ? (q % 2) * 32 + lane : q * 32 + lane;
             const int n = t * rows + r;
             const bool live = r < rows && n < N;
             const T* b = GATED && q >= 2 ? b1 : b0;
             const float bias = live && b != nullptr ? to_float(b[n]) : 0.f;
-            if (ok) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[buf], (local >> 1) & 1, bars.abort_flag));
-                if (!ok && lane == 0) atomicExch(status, 855);
-            }
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * 128;
-#pragma unroll 1
-            for (int c = 0; c < (cols + 31) / 32; c++) {
-                uint32_t v[32];
-                if (ok) {
-                    tmem_ld_32x32b_x32(taddr + c * 32, v);
-                    tmem_ld_wait();
-                }
-                if (split > 1) {   // this CTA's part, where the weights were
-                    float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+            const unsigned short* sp = reinterpret_cast<const unsigned short*>(GATED && q >= 2 ? s1 : s0) + min(n, N - 1);
+            const int groups = (K + G - 1) / G;
+            // Scales of AHEAD blocks, and of the AHEAD behind them under way: a block takes less time than a load, and loads
+            // between the uses of earlier ones would make those wait for them.
+            constexpr int AHEAD = 8 / PER;
+            unsigned short now[AHEAD][PER], next[AHEAD][PER];
+            auto load = [&](int blk) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c * 32 + i < cols) part[(c * 32 + i) * 128] = __uint_as_float(v[i]);
-                    continue;
-                }
-                if constexpr (GATED) {
-                    if (q >= 2 && ok) {
+                for (int u = 0; u < AHEAD; u++)
 #pragma unroll
-                        for (int i = 0; i < 32; i++) swap[i * 64 + r] = __uint_as_float(v[i]) + bias;
+                    for (int k = 0; k < PER; k++) next[u][k] = __ldg(sp + (size_t)min((blk0 + blk + u) * PER + k, groups - 1) * N);
+            };
+            load(0);
+            float sum[64];
+#pragma unroll
+            for (int i = 0; i < 64; i++) sum[i] = 0.f;
+            auto add = [&](unsigned short (&scales)[PER]) {   // the products of the next block
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[acc], phase_acc, bars.abort_flag));
+                    if (!ok) return;
+                    tc_fence_after();
+                    const float s = __half2float(__ushort_as_half(scales[k]));
+                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 128 + col0;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {   // 32 columns, or 16 where there are no more
+                        uint32_t v[2][16];
+                        if (c * 32 < width) tmem_ld_32x32b_x16(taddr + c * 32, v[0]);
+                        if (c * 32 + 16 < width) tmem_ld_32x32b_x16(taddr + c * 32 + 16, v[1]);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            if (c * 32 + e * 16 < width) {
+#pragma unroll
+                                for (int i = 0; i < 16; i++)
+                                    sum[c * 32 + e * 16 + i] = fmaf(__uint_as_float(v[e][i]), s, sum[c * 32 + e * 16 + i]);
+                            }
                     }
-                    named_barrier_sync(1, kEpiThreads);
-                    if (q < 2 && ok) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.tmem_empty[acc]);
+                    if (++acc == kAccs) {
+                        acc = 0;
+                        phase_acc ^= 1;
+                    }
+                }
+            };
+            for (int blk = 0; blk < blocks && ok; blk += AHEAD) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const int m = c * 32 + i;
-                            if (live && m < M)
-                                out[(size_t)m * N + n] = from_float<T>(silu_mul(__uint_as_float(v[i]) + bias, swap[i * 64 + r]));
+                for (int i = 0; i < AHEAD * PER; i++) now[i / PER][i % PER] = next[i / PER][i % PER];
+                load(blk + AHEAD);
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    if (blk + u < blocks && ok) add(now[u]);
+            }
+            if (!ok && lane == 0) atomicExch(status, 855);
+            if (split > 1) {   // this CTA's part, where the weights were
+                float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < 64; i++)
+                    if (i < width) part[(col0 + i) * 128] = sum[i];
+                continue;
+            }
+            if constexpr (GATED) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {   // 16 tokens of each half at a time
+                    if (c * 16 < width) {
+                        if (q >= 2) {
+#pragma unroll
+                            for (int i = 0; i < 16; i++) swap[(half * 16 + i) * 64 + r] = sum[c * 16 + i] + bias;
                         }
-                    }
-                    named_barrier_sync(1, kEpiThreads);
-                } else if (ok) {
+                        named_barrier_sync(1, 32 * kSumWarps);
+                        if (q < 2) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const int m = c * 32 + i;
-                        if (live && m < M) out[(size_t)m * N + n] = from_float<T>(__uint_as_float(v[i]) + bias);
+                            for (int i = 0; i < 16; i++) {
+                                const int m = col0 + c * 16 + i;
+                                if (live && m < M && ok)
+                                    out[(size_t)m * N + n] = from_float<T>(silu_mul(sum[c * 16 + i] + bias, swap[(half * 16 + i) * 64 + r]));
+                            }
+                        }
+                        named_barrier_sync(1, 32 * kSumWarps);
                     }
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 64; i++)
+                    if (i < width && live && col0 + i < M && ok)
+                        out[(size_t)(col0 + i) * N + n] = from_float<T>(sum[i] + bias);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.tmem_empty[buf]);
         }
     }
 
@@ -710,7 +792,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     __syncthreads();
     if (warp_id == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 256);
+        tmem_dealloc(tmem_base, 128 * kAccs);
     }
     if (split > 1) {
         cluster_sync_all();   // all parts are there
@@ -730,7 +812,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             };
             // every split-th token is this CTA's
             constexpr int LANES = GATED ? 64 : 128;
-            for (int i = threadIdx.x; i < (M - rank + split - 1) / split * LANES; i += kThreads) {
+            for (int i = threadIdx.x; i < (M - rank + split - 1) / split * LANES; i += kTokenThreads) {
                 const int m = rank + i / LANES * split, r = i % LANES, n = first_tile * rows + r;
                 if (r < rows && n < N) {
                     float v = sum(m, r) + (b0 != nullptr ? to_float(b0[n]) : 0.f);
@@ -756,7 +838,7 @@ int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __h
             return kLaunchFailed;
         ready[dev & 63] = true;
     }
-    const int cols = (M + 15) / 16 * 16;
+    const int cols = (M + 31) / 32 * 32;
     const int ring_x = std::min((kMaxSmem - kFixed) / (2 * cols * 128), kMaxRingX);
     const int most = GATED ? 64 : 128, sms = sm_count(), blocks = (K + 127) / 128;
     const long long full = ((long long)N + most - 1) / most;   // tiles of as many rows as the lanes hold
@@ -777,7 +859,7 @@ int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __h
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(split > 1 ? tiles * split : std::min(tiles, sms), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(kTokenThreads, 1, 1);
     cfg.dynamicSmemBytes = kFixed + ring_x * 2 * cols * 128;
     cfg.stream = stream;
     cfg.attrs = attr;
@@ -792,7 +874,7 @@ template <typename T, int G, bool GATED, int BN>
 int launch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
            const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
     static int max_pairs[64] = {};
-    constexpr int TILE_N = GATED ? BN / 2 : BN;
+    constexpr int TILE_N = GATED ? BN / 4 : BN;
     const CUtensorMapDataType type = type16(std::is_same<T, __nv_bfloat16>::value);
     const int tma_out = N % 8 == 0 && aligned16(out);
     CUtensorMap tm_x, tm_out;
@@ -814,14 +896,12 @@ int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* 
     if (M <= kTokensMax)
         return gated ? launch_tokens<T, G, true>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
                      : launch_tokens<T, G, false>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    if (gated) return launch<T, G, true, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     // 128 weight rows a tile take 0.6 of the time of 256 (tensor instructions of 128 columns run at their floor of 86
     // clocks): where even those leave pairs without a tile
-    const long long wide = ((long long)M + 255) / 256 * (((long long)N * (gated ? 2 : 1) + 255) / 256);
-    if (2 * wide <= sm_count() / 2)
-        return gated ? launch<T, G, true, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                     : launch<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
-    return gated ? launch<T, G, true, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                 : launch<T, G, false, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    const long long wide = ((long long)M + 255) / 256 * (((long long)N + 255) / 256);
+    return 2 * wide <= sm_count() / 2 ? launch<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                                      : launch<T, G, false, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
 }
 
 }  // namespace

@@ -246,13 +246,14 @@ int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, vo
                               int group_size, forge_stream_t stream);
 
 /* output (M,N) = x (M,K) W^T + bias (N, may be NULL); x, bias and output of `dtype` (FORGE_DTYPE_F16 or _BF16). Sums in
- * fp32, one rounding at the end; with more than 16 tokens scale * q is first rounded to `dtype` (it must be in its range). Needs K % 8 == 0, 16-byte aligned x and w_int4, 4-byte aligned w_scale
+ * fp32, one rounding at the end; with more than 128 tokens scale * q is first rounded to `dtype`, in
+ * whose range it has to be. Needs K % 8 == 0, 16-byte aligned x and w_int4, 4-byte aligned w_scale
  * (FORGE_B200_BAD_SHAPE otherwise). */
 int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale, const void* bias, void* output, int M,
                       int K, int N, int group_size, int dtype, forge_stream_t stream);
 
 /* output (M,N) = SiLU(x Wg^T + bg) * (x Wu^T + bu) with both weights in that form, in one kernel: the gate of a 4-bit
- * MLP. Arguments and preconditions as above. */
+ * MLP. Arguments and preconditions as above; scale * q is not rounded for any number of tokens. */
 int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t* wu_int4, const void* wg_scale,
                             const void* wu_scale, const void* bg, const void* bu, void* output, int M, int K, int N,
                             int group_size, int dtype, forge_stream_t stream);

@@ -106,12 +106,18 @@ def test_int4_linear(M, K, N, group, dtype):
     R.close_rounded(y, *linear_bound(x, w, s, bias, group))
 
 
-def linear_bound(x, w, s, b, group):
-    """Up to 16 tokens as R.int4_sizes says; above a weight is rounded once to the activations' type."""
+def linear_bound(x, w, s, b, group, gated=False):
+    """Up to 16 tokens as R.int4_sizes says; up to 128 integers and exact scales, a group at a time; above, a plain call's
+    weight is rounded once to the activations' type, a gated one's is in two parts, whose sum is exact."""
     K = x.shape[1]
     weight = R.unpack_int4(w, s, K, group)
     if x.shape[0] <= 16:
         return R.linear(x, weight, b, R.int4_sizes(s, K, group, x.dtype), group)
+    if x.shape[0] <= 128:
+        return R.linear(x, weight, b, None, group)
+    if gated:
+        y, err = R.linear(x, weight, b, weight.abs() * (1 + torch.finfo(x.dtype).eps))
+        return y, err + 2.0 ** -24 * (y.abs() + err)   # the sum of the two
     y, err = R.linear(x, weight, b)
     return y, err + x.double().abs() @ R.half_step(weight, x.dtype).t()
 
@@ -126,11 +132,11 @@ def test_int4_gated_linear(M, K, N, group, dtype):
     bg, bu = ((torch.randn(N, generator=g) * 0.3).to(TYPES[dtype]).to(DEV) if (M + N) % 2 else None for _ in range(2))
     h = C.int4_gated_linear(x, wg, wu, sg, su, bg, bu, group)
     _ok()
-    R.close_rounded(h, *R.gate_of(linear_bound(x, wg, sg, bg, group), linear_bound(x, wu, su, bu, group)))
+    R.close_rounded(h, *R.gate_of(linear_bound(x, wg, sg, bg, group, True), linear_bound(x, wu, su, bu, group, True)))
 
 
 @pytest.mark.parametrize("group", [32, 128])
-@pytest.mark.parametrize("M,K,N", [(1, 16384, 20000), (9, 8200, 13001), (40, 4104, 30001)])
+@pytest.mark.parametrize("M,K,N", [(1, 16384, 20000), (9, 8200, 13001), (40, 4104, 30001), (97, 1160, 20001), (150, 4104, 30001)])
 def test_several_passes_over_the_rows(M, K, N, group):
     """More rows than the SMs hold at a time, more columns than a ring."""
     g = torch.Generator().manual_seed(K)
@@ -142,7 +148,7 @@ def test_several_passes_over_the_rows(M, K, N, group):
     R.close_rounded(y, *linear_bound(x, w, s, None, group))
     h = C.int4_gated_linear(x, w, w.flip(0), s, s, None, None, group)
     _ok()
-    R.close_rounded(h, *R.gate_of(linear_bound(x, w, s, None, group), linear_bound(x, w.flip(0), s, None, group)))
+    R.close_rounded(h, *R.gate_of(linear_bound(x, w, s, None, group, True), linear_bound(x, w.flip(0), s, None, group, True)))
 
 
 @pytest.mark.parametrize("M", [1, 8, 40])

@@ -449,30 +449,37 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 // distributed shared memory, in rank order (4096 x 14336, 64 tokens: 61 us without, 30 with).
 //
 // With so few columns there is time to keep the sums exact: the operand holds the integers, every group of inputs has
-// accumulator columns of its own (a ring of four), and eight warps multiply them by the scale of their lane's row and
-// add them up in registers, in fp32. Nothing is rounded before the result.
+// accumulator columns of its own (a ring of four or eight), and eight warps multiply them by the scale of their lane's
+// row and add them up in registers, in fp32. Nothing is rounded before the result.
+//
+// Waiting for three barriers and issuing eight tensor instructions, one after the other, takes a thread twice the time of
+// the instructions, so two threads issue, one every other block. Rings have even numbers of stages: a barrier's parity
+// tells a lap from its neighbours only, so whoever waits on one has to see every lap of it.
 struct TokenBars {
-    uint64_t *full_w, *empty_w;   // [kRing]: the stage's weight warps; committed by the MMA thread
+    uint64_t *full_w, *empty_w;   // [kTokenRing]: the stage's weight warps; committed by the MMA thread
     uint64_t *full_x, *empty_x;   // [kMaxRingX]
-    uint64_t *tmem_full, *tmem_empty;   // [kAccs]
+    uint64_t *tmem_full, *tmem_empty;   // [kMaxAccs]
     uint32_t* tmem_slot;
     volatile int* abort_flag;
 };
 constexpr int kMaxRingX = 8;
-constexpr int kAccs = 4;                  // accumulators of up to 128 columns
-constexpr int kSumWarps = 8;              // two for each quarter of the lanes, half of the columns each
+constexpr int kMaxAccs = 8;               // accumulators: 8 of 64 columns, or 4 of 128
+constexpr int kTokenRing = 4;             // weight stages
 constexpr int kTokenGroupWarps = 2;       // that make a stage's weights
-constexpr int kTokenThreads = 32 * (2 + kSumWarps + kRing * kTokenGroupWarps);
+constexpr int kSumWarps = 8;              // two for each quarter of the lanes, half of the columns each
+constexpr int kFirstSum = 3;              // warps: TMA, two MMA issuers, sums, weights
+constexpr int kFirstWeight = kFirstSum + kSumWarps;
+constexpr int kTokenThreads = 32 * (kFirstWeight + kTokenRing * kTokenGroupWarps);
 constexpr int kSwapBytes = 32 * 64 * 4;   // gated: the up products of 32 tokens x 64 rows
 __device__ __forceinline__ TokenBars carve_tokens(uint8_t* p) {
     TokenBars b;
     b.full_w = reinterpret_cast<uint64_t*>(p);
-    b.empty_w = b.full_w + kRing;
-    b.full_x = b.empty_w + kRing;
+    b.empty_w = b.full_w + kTokenRing;
+    b.full_x = b.empty_w + kTokenRing;
     b.empty_x = b.full_x + kMaxRingX;
     b.tmem_full = b.empty_x + kMaxRingX;
-    b.tmem_empty = b.tmem_full + kAccs;
-    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + kAccs);
+    b.tmem_empty = b.tmem_full + kMaxAccs;
+    b.tmem_slot = reinterpret_cast<uint32_t*>(b.tmem_empty + kMaxAccs);
     b.abort_flag = reinterpret_cast<volatile int*>(b.tmem_slot + 1);
     return b;
 }
@@ -488,7 +495,8 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
-template <typename T, int G, bool GATED>
+// MAX_COLS: 64 or 128
+template <typename T, int G, bool GATED, int MAX_COLS>
 __global__ void __launch_bounds__(kTokenThreads, 1)
 int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
                    const __half* __restrict__ s0, const __half* __restrict__ s1, const T* __restrict__ b0,
@@ -498,7 +506,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     constexpr int PER = 128 / G;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int slab_x = cols * 128;
-    uint8_t* smem_x = smem + kRing * 2 * kSlab;
+    uint8_t* smem_x = smem + kTokenRing * 2 * kSlab;
     uint8_t* smem_swap = smem_x + ring_x * 2 * slab_x;
     const TokenBars bars = carve_tokens(smem_swap + kSwapBytes);
 
@@ -517,7 +525,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     const int blocks = (int)((long long)all_blocks * (rank + 1) / split) - blk0;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kRing; s++) {
+        for (int s = 0; s < kTokenRing; s++) {
             mbar_init(&bars.full_w[s], kTokenGroupWarps);
             mbar_init(&bars.empty_w[s], 1);
         }
@@ -525,7 +533,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             mbar_init(&bars.full_x[s], 1);
             mbar_init(&bars.empty_x[s], 1);
         }
-        for (int i = 0; i < kAccs; i++) {
+        for (int i = 0; i < kMaxAccs; i++) {
             mbar_init(&bars.tmem_full[i], 1);
             mbar_init(&bars.tmem_empty[i], kSumWarps);
         }
@@ -533,13 +541,14 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         fence_mbar_init();
     }
     if (warp_id == 1) {
-        tmem_alloc(bars.tmem_slot, 128 * kAccs);
+        tmem_alloc(bars.tmem_slot, 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *bars.tmem_slot;
+    constexpr int accs = 512 / MAX_COLS, acc_cols = MAX_COLS;
 
     if (warp_id == 0) {
         // ------------------------------------------------------------------ activations (TMA)
@@ -565,65 +574,53 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                 }
             }
         }
-    } else if (warp_id == 1) {
-        // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
+    } else if (warp_id == 1 || warp_id == 2) {
+        // ------------------------------------------------------------------ MMA issuers: of every other block, or one of all
+        // where a block's groups take all accumulators
+        constexpr int issuers = accs >= 2 * PER ? 2 : 1;
+        if (lane == 0 && warp_id <= issuers) {
             const uint32_t idesc = idesc_f16(128, cols, BF16, false, false);
-            int stage = 0, stage_x = 0, acc = 0;
-            uint32_t phase = 0, phase_x = 0, phase_acc = 0;
+            const int total = (num_tiles - first_tile + tile_step - 1) / tile_step * blocks;   // blocks of all tiles
             bool ok = true;
-            for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
-                for (int blk = 0; blk < blocks && ok; blk++) {
-                    if (!mbar_wait(&bars.full_x[stage_x], phase_x, bars.abort_flag) ||
-                        !mbar_wait(&bars.full_w[stage], phase, bars.abort_flag)) {
-                        atomicExch(status, 853);
+            for (int i = warp_id - 1; i < total && ok; i += issuers) {
+                const int stage = i % kTokenRing, stage_x = i & (ring_x - 1);
+                if (!mbar_wait(&bars.full_x[stage_x], (i / ring_x) & 1, bars.abort_flag) ||
+                    !mbar_wait(&bars.full_w[stage], (i / kTokenRing) & 1, bars.abort_flag)) {
+                    atomicExch(status, 853);
+                    break;
+                }
+                tc_fence_after();
+                const uint64_t da = make_desc_sw128(smem_u32(smem + stage * 2 * kSlab));
+                const uint64_t db = make_desc_sw128(smem_u32(smem_x + stage_x * 2 * slab_x));
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    const int a = i * PER + k, acc = a & (accs - 1);
+                    if (!mbar_wait(&bars.tmem_empty[acc], ((a / accs) & 1) ^ 1, bars.abort_flag)) {
+                        atomicExch(status, 852);
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t da = make_desc_sw128(smem_u32(smem + stage * 2 * kSlab));
-                    const uint64_t db = make_desc_sw128(smem_u32(smem_x + stage_x * 2 * slab_x));
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        if (k % (G / 16) == 0) {
-                            if (!mbar_wait(&bars.tmem_empty[acc], phase_acc ^ 1, bars.abort_flag)) {
-                                atomicExch(status, 852);
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                        }
-                        umma_f16(tmem_base + acc * 128, da + (k / 4) * (kSlab >> 4) + 2 * (k % 4),
-                                 db + (k / 4) * (slab_x >> 4) + 2 * (k % 4), idesc, k % (G / 16) != 0 ? 1u : 0u);
-                        if (k % (G / 16) == G / 16 - 1) {
-                            tc_commit(&bars.tmem_full[acc]);
-                            if (++acc == kAccs) {
-                                acc = 0;
-                                phase_acc ^= 1;
-                            }
-                        }
+                    for (int e = 0; e < G / 16; e++) {
+                        const int step = k * (G / 16) + e;   // of the block's eight
+                        umma_f16(tmem_base + acc * acc_cols, da + (step / 4) * (kSlab >> 4) + 2 * (step % 4),
+                                 db + (step / 4) * (slab_x >> 4) + 2 * (step % 4), idesc, e != 0 ? 1u : 0u);
                     }
-                    tc_commit(&bars.empty_w[stage]);
-                    tc_commit(&bars.empty_x[stage_x]);
-                    if (++stage == kRing) {
-                        stage = 0;
-                        phase ^= 1;
-                    }
-                    if (++stage_x == ring_x) {
-                        stage_x = 0;
-                        phase_x ^= 1;
-                    }
+                    tc_commit(&bars.tmem_full[acc]);
                 }
+                tc_commit(&bars.empty_w[stage]);
+                tc_commit(&bars.empty_x[stage_x]);
             }
         }
-    } else if (warp_id >= 2 + kSumWarps) {
+    } else if (warp_id >= kFirstWeight) {
         // ------------------------------------------------------------------ weights, as in int4_pair_kernel, unscaled
         constexpr int ROWS = 128 / (8 * kTokenGroupWarps);   // of a lane; the last ones only where a CTA has so many
         constexpr int STEP = 8 * kTokenGroupWarps;
         const int t4 = lane & 3;
         const int row8 = (lane >> 3) | ((lane >> 2) & 1) << 2;
-        const int stage = (warp_id - 2 - kSumWarps) / kTokenGroupWarps;
-        const int local_row = (warp_id - 2 - kSumWarps) % kTokenGroupWarps * 8 + row8;
+        const int stage = (warp_id - kFirstWeight) / kTokenGroupWarps;
+        const int local_row = (warp_id - kFirstWeight) % kTokenGroupWarps * 8 + row8;
         uint32_t phase = 0;
         bool ok = true;
         int blk = stage;   // of its tile
@@ -644,14 +641,14 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     if (used(i)) next[i] = __ldg(reinterpret_cast<const uint4*>(wp[i] + (size_t)b * 64));
             };
             load(min(blk, blocks - 1));
-            for (; blk < blocks; blk += kRing) {
+            for (; blk < blocks; blk += kTokenRing) {
                 // All of the next block's loads behind all uses of this one's: a load between two uses makes the second
                 // wait for it (870 clocks a row).
                 uint4 cur[ROWS];
 #pragma unroll
                 for (int i = 0; i < ROWS; i++)
                     if (used(i)) cur[i] = next[i];
-                load(min(blk + kRing, blocks - 1));
+                load(min(blk + kTokenRing, blocks - 1));
                 ok = __all_sync(0xffffffffu, mbar_wait(&bars.empty_w[stage], phase ^ 1, bars.abort_flag));
                 if (!ok) {
                     if (lane == 0) atomicExch(status, 854);
@@ -679,7 +676,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         }
     } else {
         // ------------------------------------------------------------------ sums: a lane has a row's products with half of the tokens
-        const int q = warp_id & 3, half = (warp_id - 2) / 4;
+        const int q = warp_id & 3, half = (warp_id - kFirstSum) / 4;
         const int width = cols / 2, col0 = half * width;   // a multiple of 16, at most 64
         float* swap = reinterpret_cast<float*>(smem_swap);
         int acc = 0;
@@ -695,7 +692,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             const int groups = (K + G - 1) / G;
             // Scales of AHEAD blocks, and of the AHEAD behind them under way: a block takes less time than a load, and loads
             // between the uses of earlier ones would make those wait for them.
-            constexpr int AHEAD = 8 / PER;
+            constexpr int AHEAD = (MAX_COLS > 64 ? 4 : 8) / PER;   // as the registers allow
             unsigned short now[AHEAD][PER], next[AHEAD][PER];
             auto load = [&](int blk) {
 #pragma unroll
@@ -704,9 +701,10 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     for (int k = 0; k < PER; k++) next[u][k] = __ldg(sp + (size_t)min((blk0 + blk + u) * PER + k, groups - 1) * N);
             };
             load(0);
-            float sum[64];
+            constexpr int SUMS = MAX_COLS / 2;
+            float sum[SUMS];
 #pragma unroll
-            for (int i = 0; i < 64; i++) sum[i] = 0.f;
+            for (int i = 0; i < SUMS; i++) sum[i] = 0.f;
             auto add = [&](unsigned short (&scales)[PER]) {   // the products of the next block
 #pragma unroll
                 for (int k = 0; k < PER; k++) {
@@ -714,25 +712,29 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     if (!ok) return;
                     tc_fence_after();
                     const float s = __half2float(__ushort_as_half(scales[k]));
-                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * 128 + col0;
+                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * acc_cols + col0;
+                    constexpr int CHUNK = SUMS > 32 ? 16 : 32;   // columns at a time, as the registers allow
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {   // 32 columns, or 16 where there are no more
-                        uint32_t v[2][16];
-                        if (c * 32 < width) tmem_ld_32x32b_x16(taddr + c * 32, v[0]);
-                        if (c * 32 + 16 < width) tmem_ld_32x32b_x16(taddr + c * 32 + 16, v[1]);
-                        tmem_ld_wait();
+                    for (int c = 0; c < SUMS / CHUNK; c++) {
+                        // columns past `width` may hold anything: theirs are sums that nobody takes
+                        uint32_t v[CHUNK];
+                        if (c * CHUNK < width) {
+                            if constexpr (CHUNK == 16) tmem_ld_32x32b_x16(taddr + c * CHUNK, v);
+                            else tmem_ld_32x32b_x32(taddr + c * CHUNK, v);
+                            tmem_ld_wait();
+                        }
+                        if (c == SUMS / CHUNK - 1) {   // all of it is in registers
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&bars.tmem_empty[acc]);
+                        }
+                        if (c * CHUNK < width) {
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (c * 32 + e * 16 < width) {
-#pragma unroll
-                                for (int i = 0; i < 16; i++)
-                                    sum[c * 32 + e * 16 + i] = fmaf(__uint_as_float(v[e][i]), s, sum[c * 32 + e * 16 + i]);
-                            }
+                            for (int e = 0; e < CHUNK; e++)
+                                sum[c * CHUNK + e] = fmaf(__uint_as_float(v[e]), s, sum[c * CHUNK + e]);
+                        }
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.tmem_empty[acc]);
-                    if (++acc == kAccs) {
+                    if (++acc == accs) {
                         acc = 0;
                         phase_acc ^= 1;
                     }
@@ -750,13 +752,13 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             if (split > 1) {   // this CTA's part, where the weights were
                 float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
 #pragma unroll
-                for (int i = 0; i < 64; i++)
+                for (int i = 0; i < SUMS; i++)
                     if (i < width) part[(col0 + i) * 128] = sum[i];
                 continue;
             }
             if constexpr (GATED) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {   // 16 tokens of each half at a time
+                for (int c = 0; c < SUMS / 16; c++) {   // 16 tokens of each half at a time
                     if (c * 16 < width) {
                         if (q >= 2) {
 #pragma unroll
@@ -776,7 +778,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 64; i++)
+                for (int i = 0; i < SUMS; i++)
                     if (i < width && live && col0 + i < M && ok)
                         out[(size_t)(col0 + i) * N + n] = from_float<T>(sum[i] + bias);
             }
@@ -792,7 +794,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     __syncthreads();
     if (warp_id == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, 128 * kAccs);
+        tmem_dealloc(tmem_base, 512);
     }
     if (split > 1) {
         cluster_sync_all();   // all parts are there
@@ -825,12 +827,12 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     }
 }
 
-template <typename T, int G, bool GATED>
+template <typename T, int G, bool GATED, int MAX_COLS>
 int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
                   const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
     static bool ready[64] = {};
-    auto kern = int4_tokens_kernel<T, G, GATED>;
-    constexpr int kMaxSmem = 227 * 1024, kFixed = kRing * 2 * kSlab + kSwapBytes + 512;
+    auto kern = int4_tokens_kernel<T, G, GATED, MAX_COLS>;
+    constexpr int kMaxSmem = 227 * 1024, kFixed = kTokenRing * 2 * kSlab + kSwapBytes + 512;
     int dev = 0;
     cudaGetDevice(&dev);
     if (!ready[dev & 63]) {
@@ -839,7 +841,8 @@ int launch_tokens(const void* x, const uint8_t* w0, const uint8_t* w1, const __h
         ready[dev & 63] = true;
     }
     const int cols = (M + 31) / 32 * 32;
-    const int ring_x = std::min((kMaxSmem - kFixed) / (2 * cols * 128), kMaxRingX);
+    int ring_x = kMaxRingX;   // a power of two
+    while (ring_x * 2 * cols * 128 > kMaxSmem - kFixed) ring_x /= 2;
     const int most = GATED ? 64 : 128, sms = sm_count(), blocks = (K + 127) / 128;
     const long long full = ((long long)N + most - 1) / most;   // tiles of as many rows as the lanes hold
     int split = 1;
@@ -893,9 +896,12 @@ template <typename T, int G>
 int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
              const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
     const bool gated = w1 != nullptr;
+    if (M <= 64)
+        return gated ? launch_tokens<T, G, true, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                     : launch_tokens<T, G, false, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     if (M <= kTokensMax)
-        return gated ? launch_tokens<T, G, true>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                     : launch_tokens<T, G, false>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+        return gated ? launch_tokens<T, G, true, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                     : launch_tokens<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     if (gated) return launch<T, G, true, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     // 128 weight rows a tile take 0.6 of the time of 256 (tensor instructions of 128 columns run at their floor of 86
     // clocks): where even those leave pairs without a tile

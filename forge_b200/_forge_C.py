@@ -203,16 +203,36 @@ def int8_conv_transpose2d_k2s2_forward(input, weight, w_scale, bias):
 
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # FORGE_DTYPE_*
+_DTYPES16 = {torch.float16: 1, torch.bfloat16: 2}
+_GROUPS = (32, 64, 128)
 _BYTES_PER_BLOCK = 64   # packed 4-bit weights: 128 inputs
 
 
-def _act_dtype(x):
-    """FORGE_DTYPE_* of a 2-D fp16 / bf16 activation whose row length the kernels take."""
-    if x.dtype not in (torch.float16, torch.bfloat16):
+def _act_shape(x):
+    """FORGE_DTYPE_* and shape of a contiguous 2-D fp16 / bf16 CUDA activation whose row length the kernels take."""
+    dtype = _DTYPES16.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"x: expected torch.float16 or torch.bfloat16, got {x.dtype}")
-    if x.dim() != 2 or x.size(1) == 0 or x.size(1) % 8 != 0:
-        raise ValueError(f"x: expected (tokens, inputs) with inputs a positive multiple of 8, got {tuple(x.shape)}")
-    return _DTYPES[x.dtype]
+    if not x.is_cuda:
+        raise ValueError("forge_b200 runs on CUDA tensors only (there is no CPU path)")
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0 or shape[1] % 8 != 0:
+        raise ValueError(f"x: expected (tokens, inputs) with inputs a positive multiple of 8, got {tuple(shape)}")
+    if not x.is_contiguous():
+        raise ValueError("x: must be contiguous")
+    return dtype, shape[0], shape[1]
+
+
+def _run(t, name, *args):
+    """An entry point on `t`'s GPU and its current stream, which goes in as the last argument."""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        status = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            _lib.check(status, name)
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream())
 
 
 def _shape(**named):
@@ -227,7 +247,7 @@ def _aligned(t):
 
 
 def _check_group(group_size):
-    if group_size not in (32, 64, 128):
+    if group_size not in _GROUPS:
         raise ValueError(f"group_size: expected 32, 64 or 128, got {group_size}")
 
 
@@ -245,91 +265,79 @@ def prepare_weight_int4(weight, group_size=128):
     N, K = weight.shape
     w_int4 = torch.empty((N, (K + 127) // 128 * _BYTES_PER_BLOCK), dtype=_u8, device=weight.device)
     w_scale = torch.empty(((K + group_size - 1) // group_size, N), dtype=_f16, device=weight.device)
-    with _on(weight):
-        _lib.call("forge_prepare_weight_int4", _ptr(weight), _DTYPES[weight.dtype], _ptr(w_int4), _ptr(w_scale), N, K,
-                  group_size, _stream())
+    _run(weight, "forge_prepare_weight_int4", _ptr(weight), _DTYPES[weight.dtype], _ptr(w_int4), _ptr(w_scale), N, K,
+         group_size)
     return w_int4, w_scale
 
 
-def _int4_operand(x, name, w, s, b, N, group_size):
-    """Checks one 4-bit weight with its scales and bias against x (M, K) and N outputs."""
-    K = x.size(1)
-    dev = x.device
-    if w.dtype != _u8 or s.dtype != _f16 or (b is not None and b.dtype != x.dtype):
+def _int4_operand(x, K, name, w, s, b, N, group_size):
+    """Checks one 4-bit weight with its scales and bias against x (M, K) and N outputs; returns their addresses."""
+    if w.dtype is not _u8 or s.dtype is not _f16 or (b is not None and b.dtype is not x.dtype):
         raise TypeError(f"{name}_int4, {name}_scale, bias: expected {_u8}, {_f16}, {x.dtype}, "
                         f"got {w.dtype}, {s.dtype}, {None if b is None else b.dtype}")
     if w.shape != (N, (K + 127) // 128 * _BYTES_PER_BLOCK) or s.shape != ((K + group_size - 1) // group_size, N) or (
             b is not None and b.shape != (N,)):
         raise ValueError(f"{name}_int4 {tuple(w.shape)}, {name}_scale {tuple(s.shape)}, bias "
                          f"{None if b is None else tuple(b.shape)} do not fit {K} inputs in groups of {group_size}, {N} outputs")
+    dev = x.device
     if w.device != dev or s.device != dev or (b is not None and b.device != dev):
         raise ValueError(f"{name}_int4, {name}_scale and bias must be on {dev}")
     if not (w.is_contiguous() and s.is_contiguous() and (b is None or b.is_contiguous())):
         raise ValueError(f"{name}_int4, {name}_scale and bias must be contiguous")
-    if w.data_ptr() % 16 != 0 or s.data_ptr() % 4 != 0:
+    pw, ps = w.data_ptr(), s.data_ptr()
+    if pw & 15 or ps & 3:
         raise ValueError(f"{name}_int4 must start at a 16-byte aligned address, {name}_scale at a 4-byte aligned one")
+    return pw, ps, 0 if b is None else b.data_ptr()
 
 
 def int4_linear(x, w_int4, w_scale, bias=None, group_size=128):
     """x (M, K) fp16 / bf16 times a 4-bit weight (prepare_weight_int4) plus bias (N) of x's type -> (M, N)."""
-    dtype = _act_dtype(x)
+    dtype, M, K = _act_shape(x)
     _check_group(group_size)
-    _chk(x, x=(x, x.dtype))
-    M, K = x.shape
-    N = w_int4.size(0)
-    _int4_operand(x, "w", w_int4, w_scale, bias, N, group_size)
+    N = w_int4.shape[0]
+    w, s, b = _int4_operand(x, K, "w", w_int4, w_scale, bias, N, group_size)
     x = _aligned(x)
     output = x.new_empty((M, N))
-    with _on(x):
-        _lib.call("forge_int4_linear", _ptr(x), _ptr(w_int4), _ptr(w_scale), _ptr(bias), _ptr(output), M, K, N,
-                  group_size, dtype, _stream())
+    _run(x, "forge_int4_linear", x.data_ptr(), w, s, b, output.data_ptr(), M, K, N, group_size, dtype)
     return output
 
 
 def int4_gated_linear(x, wg_int4, wu_int4, wg_scale, wu_scale, bg=None, bu=None, group_size=128):
     """SiLU(x Wg^T + bg) * (x Wu^T + bu) for 4-bit weights, one kernel -> (M, N)."""
-    dtype = _act_dtype(x)
+    dtype, M, K = _act_shape(x)
     _check_group(group_size)
-    _chk(x, x=(x, x.dtype))
-    M, K = x.shape
-    N = wg_int4.size(0)
-    _int4_operand(x, "wg", wg_int4, wg_scale, bg, N, group_size)
-    _int4_operand(x, "wu", wu_int4, wu_scale, bu, N, group_size)
+    N = wg_int4.shape[0]
+    wg, sg, pg = _int4_operand(x, K, "wg", wg_int4, wg_scale, bg, N, group_size)
+    wu, su, pu = _int4_operand(x, K, "wu", wu_int4, wu_scale, bu, N, group_size)
     x = _aligned(x)
     output = x.new_empty((M, N))
-    with _on(x):
-        _lib.call("forge_int4_gated_linear", _ptr(x), _ptr(wg_int4), _ptr(wu_int4), _ptr(wg_scale), _ptr(wu_scale),
-                  _ptr(bg), _ptr(bu), _ptr(output), M, K, N, group_size, dtype, _stream())
+    _run(x, "forge_int4_gated_linear", x.data_ptr(), wg, wu, sg, su, pg, pu, output.data_ptr(), M, K, N, group_size, dtype)
     return output
 
 
 def gated_linear(x, Wg, Wu, bg=None, bu=None, save=False):
     """SiLU(x Wg^T + bg) * (x Wu^T + bu) for fp16 / bf16 weights (N, K) -> (M, N). save=True: also the two products in
     fp32, (h, g, u), which gated_linear_backward takes. No autograd; see forge_b200.nn.gated_linear."""
-    dtype = _act_dtype(x)
-    M, K = x.shape
-    N = Wg.size(0)
-    _chk(x, x=(x, x.dtype), Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), bg=(bg, x.dtype), bu=(bu, x.dtype))
+    dtype, M, K = _act_shape(x)
+    N = Wg.shape[0]
+    _chk(x, Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), bg=(bg, x.dtype), bu=(bu, x.dtype))
     _shape(Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), bg=(bg, (N,)), bu=(bu, (N,)))
     if N % 8 != 0:
         raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, got {N}")
     x, Wg, Wu = _aligned(x), _aligned(Wg), _aligned(Wu)
-    h = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    h = x.new_empty((M, N))
     g = u = None
     if save:
-        g = torch.empty((M, N), dtype=_f32, device=x.device)
-        u = torch.empty((M, N), dtype=_f32, device=x.device)
-    with _on(x):
-        _lib.call("forge_gated_linear", _ptr(x), _ptr(Wg), _ptr(Wu), _ptr(bg), _ptr(bu), _ptr(h), _ptr(g), _ptr(u), M, K,
-                  N, dtype, _stream())
+        g, u = x.new_empty((M, N), dtype=_f32), x.new_empty((M, N), dtype=_f32)
+    _run(x, "forge_gated_linear", x.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), _ptr(g),
+         _ptr(u), M, K, N, dtype)
     return (h, g, u) if save else h
 
 
 def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=True):
     """Gradients of gated_linear for dh (M, N): (dx, dWg, dWu, dbg, dbu) in x's type, None where not asked for."""
-    dtype = _act_dtype(x)
-    M, K = x.shape
-    N = Wg.size(0)
+    dtype, M, K = _act_shape(x)
+    N = Wg.shape[0]
     _chk(x, dh=(dh, x.dtype), x=(x, x.dtype), Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), g=(g, _f32), u=(u, _f32))
     _shape(dh=(dh, (M, N)), Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), g=(g, (M, N)), u=(u, (M, N)))
     if N % 8 != 0:
@@ -341,11 +349,10 @@ def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=
     dbg, dbu = (new((N,), dtype=x.dtype, device=x.device) if need_b else None for _ in range(2))
     dh, x, Wg, Wu = _aligned(dh), _aligned(x), _aligned(Wg), _aligned(Wu)
     g, u = _aligned(g), _aligned(u)
-    with _on(x):
-        size = _lib.load().forge_gated_linear_backward_workspace_bytes(M, N)
-        workspace = torch.empty((size,), dtype=_u8, device=x.device)
-        _lib.call("forge_gated_linear_backward", _ptr(dh), _ptr(x), _ptr(Wg), _ptr(Wu), _ptr(g), _ptr(u), _ptr(dx),
-                  _ptr(dWg), _ptr(dWu), _ptr(dbg), _ptr(dbu), M, K, N, dtype, _ptr(workspace), _stream())
+    size = _lib.load().forge_gated_linear_backward_workspace_bytes(M, N)
+    workspace = torch.empty((size,), dtype=_u8, device=x.device)
+    _run(x, "forge_gated_linear_backward", _ptr(dh), _ptr(x), _ptr(Wg), _ptr(Wu), _ptr(g), _ptr(u), _ptr(dx), _ptr(dWg),
+         _ptr(dWu), _ptr(dbg), _ptr(dbu), M, K, N, dtype, _ptr(workspace))
     return dx, dWg, dWu, dbg, dbu
 
 

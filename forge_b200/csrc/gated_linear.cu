@@ -292,7 +292,7 @@ gated_pair_kernel(const __grid_constant__ Maps maps, const void* __restrict__ bi
 
 constexpr int kGateRows = 64;   // tokens per CTA
 
-// A CTA takes 256 channels x kGateRows tokens: 32 threads across (8 channels each), 8 down. Bound by HBM (18 bytes an
+// A CTA takes 256 channels x kGateRows tokens: 32 threads across (8 channels each), 8 down. Bound by HBM (14 bytes an
 // element). BIAS: per-CTA column sums into part (2, row chunks, N), reduced by sum_parts_kernel.
 template <typename T, bool BIAS>
 __global__ void __launch_bounds__(256)
@@ -303,34 +303,46 @@ gate_backward_kernel(const T* __restrict__ dh, const float* __restrict__ gate, c
     const long long m0 = (long long)blockIdx.y * kGateRows;
     float sg[8] = {}, su[8] = {};
     if (n < N) {
-        for (int r = ty; r < kGateRows && m0 + r < M; r += 8) {
-            const size_t at = (size_t)(m0 + r) * N + n;
-            const uint4 d4 = __ldcs(reinterpret_cast<const uint4*>(dh + at));
-            const T* d = reinterpret_cast<const T*>(&d4);
-            float g[8], u[8];
+        // two rows at a time, so that 160 bytes a thread are under way
+        for (int r0 = ty; r0 < kGateRows && m0 + r0 < M; r0 += 16) {
+            const bool two = r0 + 8 < kGateRows && m0 + r0 + 8 < M;
+            uint4 d4[2];
+            float4 g4[2][2], u4[2][2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float4 a = __ldcs(reinterpret_cast<const float4*>(gate + at) + h);
-                const float4 b = __ldcs(reinterpret_cast<const float4*>(up + at) + h);
-                g[4 * h] = a.x; g[4 * h + 1] = a.y; g[4 * h + 2] = a.z; g[4 * h + 3] = a.w;
-                u[4 * h] = b.x; u[4 * h + 1] = b.y; u[4 * h + 2] = b.z; u[4 * h + 3] = b.w;
-            }
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || two) {
+                    const size_t at = (size_t)(m0 + r0 + 8 * k) * N + n;
+                    d4[k] = __ldcs(reinterpret_cast<const uint4*>(dh + at));
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float s = __fdividef(1.f, 1.f + __expf(-g[i]));
-                const float v = to_float(d[i]);
-                const float a = v * u[i] * s * (1.f + g[i] * (1.f - s)), b = v * g[i] * s;
-                g[i] = a;
-                u[i] = b;
-                if (BIAS) {
-                    sg[i] += a;
-                    su[i] += b;
+                    for (int h = 0; h < 2; h++) {
+                        g4[k][h] = __ldcs(reinterpret_cast<const float4*>(gate + at) + h);
+                        u4[k][h] = __ldcs(reinterpret_cast<const float4*>(up + at) + h);
+                    }
                 }
-            }
-            *reinterpret_cast<uint4*>(dg + at) =
-                make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]), pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
-            *reinterpret_cast<uint4*>(du + at) =
-                make_uint4(pack2<T>(u[0], u[1]), pack2<T>(u[2], u[3]), pack2<T>(u[4], u[5]), pack2<T>(u[6], u[7]));
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || two) {
+                    const size_t at = (size_t)(m0 + r0 + 8 * k) * N + n;
+                    const T* d = reinterpret_cast<const T*>(&d4[k]);
+                    float g[8] = {g4[k][0].x, g4[k][0].y, g4[k][0].z, g4[k][0].w, g4[k][1].x, g4[k][1].y, g4[k][1].z, g4[k][1].w};
+                    float u[8] = {u4[k][0].x, u4[k][0].y, u4[k][0].z, u4[k][0].w, u4[k][1].x, u4[k][1].y, u4[k][1].z, u4[k][1].w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float s = __fdividef(1.f, 1.f + __expf(-g[i]));
+                        const float v = to_float(d[i]);
+                        const float a = v * u[i] * s * (1.f + g[i] * (1.f - s)), b = v * g[i] * s;
+                        g[i] = a;
+                        u[i] = b;
+                        if (BIAS) {
+                            sg[i] += a;
+                            su[i] += b;
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dg + at) = make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]),
+                                                                    pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
+                    *reinterpret_cast<uint4*>(du + at) = make_uint4(pack2<T>(u[0], u[1]), pack2<T>(u[2], u[3]),
+                                                                    pack2<T>(u[4], u[5]), pack2<T>(u[6], u[7]));
+                }
         }
     }
     if constexpr (BIAS) {

@@ -206,6 +206,7 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # FORGE_DTYP
 _DTYPES16 = {torch.float16: 1, torch.bfloat16: 2}
 _GROUPS = (32, 64, 128)
 _BYTES_PER_BLOCK = 64   # packed 4-bit weights: 128 inputs
+_MAX_SIZE = 1 << 30      # of one dimension, as the library checks it
 
 
 def _act_shape(x):
@@ -218,6 +219,8 @@ def _act_shape(x):
     shape = x.shape
     if len(shape) != 2 or shape[1] == 0 or shape[1] % 8 != 0:
         raise ValueError(f"x: expected (tokens, inputs) with inputs a positive multiple of 8, got {tuple(shape)}")
+    if shape[0] > _MAX_SIZE or shape[1] > _MAX_SIZE:
+        raise ValueError(f"x: at most {_MAX_SIZE} rows and columns, got {tuple(shape)}")
     if not x.is_contiguous():
         raise ValueError("x: must be contiguous")
     return dtype, shape[0], shape[1]
@@ -322,8 +325,8 @@ def gated_linear(x, Wg, Wu, bg=None, bu=None, save=False):
     N = Wg.shape[0]
     _chk(x, Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), bg=(bg, x.dtype), bu=(bu, x.dtype))
     _shape(Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), bg=(bg, (N,)), bu=(bu, (N,)))
-    if N % 8 != 0:
-        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, got {N}")
+    if N % 8 != 0 or N > _MAX_SIZE:
+        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, at most {_MAX_SIZE}, got {N}")
     x, Wg, Wu = _aligned(x), _aligned(Wg), _aligned(Wu)
     h = x.new_empty((M, N))
     g = u = None
@@ -340,8 +343,8 @@ def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=
     N = Wg.shape[0]
     _chk(x, dh=(dh, x.dtype), x=(x, x.dtype), Wg=(Wg, x.dtype), Wu=(Wu, x.dtype), g=(g, _f32), u=(u, _f32))
     _shape(dh=(dh, (M, N)), Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), g=(g, (M, N)), u=(u, (M, N)))
-    if N % 8 != 0:
-        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, got {N}")
+    if N % 8 != 0 or N > _MAX_SIZE:
+        raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, at most {_MAX_SIZE}, got {N}")
     # without tokens the library writes nothing, and the gradients of the weights are zero
     new = torch.zeros if M == 0 else torch.empty
     dx = new((M, K), dtype=x.dtype, device=x.device) if need_x else None

@@ -55,8 +55,11 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, const __half*
 
 inline bool is_16bit(int dtype) { return dtype == FORGE_DTYPE_F16 || dtype == FORGE_DTYPE_BF16; }
 // Up to here the streaming kernel, whose cost is that of a pass over the weight for every 16 tokens, beats the kernels with
-// tensor-memory tiles: 4096 x 4096 10 against 15 us at 16 tokens, 17 against 15 at 17.
+// tensor-memory tiles: 4096 x 4096 10 against 19 us at 16 tokens, 11008 x 4096 17 against 22.
 constexpr int kInt4StreamTokens = 16;
+// Sizes of the 16-bit and 4-bit entry points: kernels round them up to tiles and multiply tile numbers, in 32 bits
+constexpr int kMaxSize = 1 << 30;
+inline bool too_large(int M, int K, int N) { return M > kMaxSize || K > kMaxSize || N > kMaxSize; }
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline bool is_group(int g) { return g == 32 || g == 64 || g == 128; }
 
@@ -310,8 +313,8 @@ int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void
     if (M <= 0 || K <= 0 || N <= 0) return kOk;
     if (x == nullptr || Wg == nullptr || Wu == nullptr || h == nullptr || (g_out == nullptr) != (u_out == nullptr))
         return kBadPointer;
-    if (K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(x) || !aligned16(Wg) || !aligned16(Wu) ||
-        !aligned16(h) || !aligned16(g_out) || !aligned16(u_out))
+    if (too_large(M, K, N) || K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(x) || !aligned16(Wg) ||
+        !aligned16(Wu) || !aligned16(h) || !aligned16(g_out) || !aligned16(u_out))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
     return gated_linear(x, Wg, Wu, bg, bu, h, g_out, u_out, M, K, N, dtype == FORGE_DTYPE_BF16, S(stream));
@@ -328,9 +331,9 @@ int forge_gated_linear_backward(const void* dh, const void* x, const void* Wg, c
     if (dh == nullptr || x == nullptr || Wg == nullptr || Wu == nullptr || g == nullptr || u == nullptr ||
         workspace == nullptr || (dWg == nullptr) != (dWu == nullptr))
         return kBadPointer;
-    if (K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(dh) || !aligned16(x) || !aligned16(Wg) ||
-        !aligned16(Wu) || !aligned16(g) || !aligned16(u) || !aligned16(dx) || !aligned16(dWg) || !aligned16(dWu) ||
-        (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    if (too_large(M, K, N) || K % 8 != 0 || N % 8 != 0 || !is_16bit(dtype) || !aligned16(dh) || !aligned16(x) ||
+        !aligned16(Wg) || !aligned16(Wu) || !aligned16(g) || !aligned16(u) || !aligned16(dx) || !aligned16(dWg) ||
+        !aligned16(dWu) || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
     return gated_linear_backward(dh, x, Wg, Wu, g, u, dx, dWg, dWu, dbg, dbu, M, K, N, dtype == FORGE_DTYPE_BF16,
@@ -341,8 +344,8 @@ int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, vo
                               int group_size, forge_stream_t stream) {
     if (N <= 0 || K <= 0) return kOk;
     if (weight == nullptr || w_int4 == nullptr || w_scale == nullptr) return kBadPointer;
-    if (K % 8 != 0 || !is_group(group_size) || dtype < FORGE_DTYPE_F32 || dtype > FORGE_DTYPE_BF16 ||
-        !aligned16(weight) || !aligned16(w_int4))
+    if (too_large(0, K, N) || K % 8 != 0 || !is_group(group_size) || dtype < FORGE_DTYPE_F32 ||
+        dtype > FORGE_DTYPE_BF16 || !aligned16(weight) || !aligned16(w_int4))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
     return prepare_weight_int4(weight, dtype, w_int4, H(w_scale), N, K, group_size, S(stream));
@@ -352,12 +355,13 @@ int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale,
                       int K, int N, int group_size, int dtype, forge_stream_t stream) {
     if (M <= 0 || K <= 0 || N <= 0) return kOk;
     if (x == nullptr || w_int4 == nullptr || w_scale == nullptr || output == nullptr) return kBadPointer;
-    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(w_int4) ||
-        !aligned4(w_scale))
+    if (too_large(M, K, N) || K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) ||
+        !aligned16(w_int4) || !aligned4(w_scale))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size,
-                       dtype == FORGE_DTYPE_BF16, S(stream));
+    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(
+        x, w_int4, nullptr, H(w_scale), nullptr, bias, nullptr, output, M, K, N, group_size, dtype == FORGE_DTYPE_BF16,
+        S(stream));
 }
 
 int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t* wu_int4, const void* wg_scale,
@@ -367,12 +371,13 @@ int forge_int4_gated_linear(const void* x, const uint8_t* wg_int4, const uint8_t
     if (x == nullptr || wg_int4 == nullptr || wu_int4 == nullptr || wg_scale == nullptr || wu_scale == nullptr ||
         output == nullptr)
         return kBadPointer;
-    if (K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) || !aligned16(wg_int4) ||
-        !aligned16(wu_int4) || !aligned4(wg_scale) || !aligned4(wu_scale))
+    if (too_large(M, K, N) || K % 8 != 0 || !is_group(group_size) || !is_16bit(dtype) || !aligned16(x) ||
+        !aligned16(wg_int4) || !aligned16(wu_int4) || !aligned4(wg_scale) || !aligned4(wu_scale))
         return kBadShape;
     if (!device_is_sm100()) return kUnsupportedArch;
-    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size,
-                       dtype == FORGE_DTYPE_BF16, S(stream));
+    return (M <= kInt4StreamTokens ? int4_stream : int4_gemm)(
+        x, wg_int4, wu_int4, H(wg_scale), H(wu_scale), bg, bu, output, M, K, N, group_size, dtype == FORGE_DTYPE_BF16,
+        S(stream));
 }
 
 int forge_prune_compress_24(const int8_t* weight, int8_t* compressed, uint8_t* metadata_raw, int N, int K,

@@ -147,6 +147,9 @@ def quantize_weight_int4(weight_fp, group_size=128):
     w = weight_fp.detach()
     if w.is_cuda:
         return _C.prepare_weight_int4(w, group_size)
+    _C._check_group(group_size)
+    if w.dim() != 2 or w.size(1) == 0 or w.size(1) % 8 != 0:
+        raise ValueError(f"weight: expected (outputs, inputs) with inputs a positive multiple of 8, got {tuple(w.shape)}")
     N, K = w.shape
     groups = -(-K // group_size)
     w = torch.nn.functional.pad(w.to(torch.float32).to(torch.float64), (0, groups * group_size - K)).view(N, groups, group_size)
@@ -159,6 +162,12 @@ def quantize_weight_int4(weight_fp, group_size=128):
     # blocks of 128: run 4j + t of eight weights is word 4t + j; weight 2i in nibble i, weight 2i + 1 in nibble i + 4
     q = q.view(N, -1, 4, 4, 4, 2).transpose(2, 3).transpose(4, 5).reshape(N, -1, 2)
     return (q[..., 0] | q[..., 1] << 4).to(torch.uint8), s.t().contiguous()
+
+
+def _check_weight(module, *weights):
+    for w in weights:
+        if w.shape != (module.out_features, module.in_features):
+            raise ValueError(f"weight: expected shape {(module.out_features, module.in_features)}, got {tuple(w.shape)}")
 
 
 def _as_16bit_rows(x, dtype):
@@ -195,6 +204,7 @@ class Int4Linear(nn.Module):
 
     @torch.no_grad()
     def quantize_weight(self, weight_fp):
+        _check_weight(self, weight_fp)
         w, s = quantize_weight_int4(weight_fp.to(self.w_int4.device), self.group_size)
         self.w_int4.copy_(w)
         self.w_scale.copy_(s)
@@ -223,7 +233,10 @@ class _GatedLinearFn(torch.autograd.Function):
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None):
     """SiLU(x w_gate^T + b_gate) * (x w_up^T + b_up), differentiable in every argument. x (..., K), weights (N, K), biases
-    (N), all fp16 or all bf16, K and N multiples of 8. In training the two products are kept in fp32."""
+    (N), all fp16 or all bf16, K and N multiples of 8. In training the two products are kept in fp32.
+
+    A step can be captured into a CUDA graph. As with every autograd operation, no graph recorded outside the capture may
+    then still be alive for the same leaves: its gradient accumulators belong to the stream it was recorded on."""
     x2 = x.reshape(-1, x.shape[-1]).contiguous()
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     args = (x2, w_gate, w_up, b_gate, b_up)
@@ -294,6 +307,7 @@ class Int4GatedLinear(nn.Module):
 
     @torch.no_grad()
     def quantize_weight(self, w_gate_fp, w_up_fp):
+        _check_weight(self, w_gate_fp, w_up_fp)
         for k, w in (("gate", w_gate_fp), ("up", w_up_fp)):
             q, s = quantize_weight_int4(w.to(self.w_gate_int4.device), self.group_size)
             getattr(self, f"w_{k}_int4").copy_(q)

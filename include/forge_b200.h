@@ -215,7 +215,8 @@ enum {
  *   g = x Wg^T + bg,  u = x Wu^T + bu,  h = SiLU(g) * u
  * x (M,K), Wg / Wu (N,K), bg / bu (N, may be NULL), h (M,N), all of `dtype` (FORGE_DTYPE_F16 or _BF16). g_out / u_out:
  * (M,N) fp32 that receive g and u for the backward pass, both or neither NULL. Products, gate and sums are evaluated in
- * fp32, h is rounded once. Needs K % 8 == 0, N % 8 == 0 and 16-byte aligned matrices (FORGE_B200_BAD_SHAPE otherwise). */
+ * fp32, h is rounded once. Needs K % 8 == 0, N % 8 == 0, sizes up to 2^30 and 16-byte aligned matrices
+ * (FORGE_B200_BAD_SHAPE otherwise). */
 int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void* bg, const void* bu, void* h,
                        float* g_out, float* u_out, int M, int K, int N, int dtype, forge_stream_t stream);
 
@@ -223,7 +224,7 @@ int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void
  * all of `dtype`; g and u as the forward call wrote them. The gradients of g and u are rounded to `dtype` before the
  * products, everything else is fp32; the order of every sum is fixed. `workspace` is caller-owned device memory of
  * forge_gated_linear_backward_workspace_bytes(M, N) bytes, 256-byte aligned. With M <= 0 nothing is written, the
- * gradients of the weights included (they are zero). */
+ * gradients of the weights included (they are zero). At most 4194240 tokens (FORGE_B200_TOO_LARGE otherwise). */
 unsigned long long forge_gated_linear_backward_workspace_bytes(int M, int N);
 int forge_gated_linear_backward(const void* dh, const void* x, const void* Wg, const void* Wu, const float* g,
                                 const float* u, void* dx, void* dWg, void* dWu, void* dbg, void* dbu, int M, int K,
@@ -247,8 +248,9 @@ int forge_prepare_weight_int4(const void* weight, int dtype, uint8_t* w_int4, vo
 
 /* output (M,N) = x (M,K) W^T + bias (N, may be NULL); x, bias and output of `dtype` (FORGE_DTYPE_F16 or _BF16). Sums in
  * fp32, one rounding at the end; with more than 128 tokens scale * q is first rounded to `dtype`, in
- * whose range it has to be. Needs K % 8 == 0, 16-byte aligned x and w_int4, 4-byte aligned w_scale
- * (FORGE_B200_BAD_SHAPE otherwise). */
+ * whose range it has to be. A token with an infinite input has NaN or infinite outputs, with up to 16 tokens NaN.
+ * Needs K % 8 == 0, sizes up to 2^30, 16-byte aligned x and w_int4, 4-byte aligned w_scale (FORGE_B200_BAD_SHAPE
+ * otherwise). */
 int forge_int4_linear(const void* x, const uint8_t* w_int4, const void* w_scale, const void* bias, void* output, int M,
                       int K, int N, int group_size, int dtype, forge_stream_t stream);
 

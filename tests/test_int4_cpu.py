@@ -145,3 +145,30 @@ def test_c_refusals():
     assert [bwd(K=12), bwd(N=4), bwd(dtype=0), bwd(ws=p + 128)] == [BAD_SHAPE] * 4
     size = lib.forge_gated_linear_backward_workspace_bytes
     assert size(0, 16) == 0 and size(4, 0) == 0 and size(8192, 14336) >= 2 * 2 * 8192 * 14336
+
+
+def test_c_refusals_of_sizes():
+    lib, p, big = _lib.load(), 0x10000, (1 << 30) + 8
+    for M, K, N in ((big, 64, 16), (4, big, 16), (4, 64, big)):
+        assert lib.forge_int4_linear(p, p, p, 0, p, M, K, N, 64, 1, 0) == BAD_SHAPE
+        assert lib.forge_int4_gated_linear(p, p, p, p, p, 0, 0, p, M, K, N, 64, 1, 0) == BAD_SHAPE
+        assert lib.forge_gated_linear(p, p, p, 0, 0, p, 0, 0, M, K, N, 1, 0) == BAD_SHAPE
+        assert lib.forge_gated_linear_backward(p, p, p, p, p, p, p, p, p, 0, 0, M, K, N, 1, p, 0) == BAD_SHAPE
+        if M != big:
+            assert lib.forge_prepare_weight_int4(p, 0, p, p, N, K, 64, 0) == BAD_SHAPE
+
+
+def test_weights_of_another_shape_are_refused():
+    """A row that would be broadcast over all outputs, among them."""
+    m, gm = Int4Linear(64, 8), Int4GatedLinear(64, 8)
+    good = torch.randn(8, 64)
+    for w in (good[:1], good[:, :8], good.t(), good[0], torch.randn(16, 64)):
+        with pytest.raises(ValueError):
+            m.quantize_weight(w)
+        with pytest.raises(ValueError):
+            gm.quantize_weight(good, w)
+    for w, group in ((good, 16), (good[:, :60], 64), (good[:, :0], 64), (good[0], 64)):
+        with pytest.raises(ValueError):
+            quantize_weight_int4(w, group)
+    m.quantize_weight(good)
+    gm.quantize_weight(good, good)

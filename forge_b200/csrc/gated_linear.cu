@@ -16,6 +16,10 @@
 // dx reads Wg, Wu and dW reads dg, du, x against their memory order; tensor cores take such 16-bit operands as they
 // lie ("MN-major": 64 channels x 8 inputs per swizzle atom), so nothing is ever transposed in memory.
 //
+// 8192 tokens, 4096 -> 14336, bf16: forward 1.20 ms (1600 TFLOP/s, the burst rate of the tensor pipe), with g and u saved
+// 1.28 ms; backward 2.9 ms, of which the elementwise part takes 265 us and the products the rest (1460 TFLOP/s). 1001
+// tokens, 1024 -> 2816, forward and backward: 93 us of GPU time, four launches of tens of tiles.
+//
 // Precision: the forward keeps g and u in fp32 for the backward - 8 bytes per element, where rounding them to 16 bits
 // would put another two roundings into every gradient. dg and du are rounded to 16 bits, which the tensor cores
 // need; the bias gradients are summed from them before that rounding, in fp32, in a fixed order.

@@ -10,13 +10,19 @@
 // whole block of 128 inputs (three of 64 KB). Making one takes longer than the tensor cores need for it, so each stage has
 // four warps of its own, three blocks being made at a time; the warps signal a barrier of their own CTA only, and one
 // thread passes CTA 1's on to the leader (with eight warps on each 64-deep slab in turn and arrivals across the cluster,
-// 2048 x 4096 x 11008 took 308 us; 142 us like this, 1300 TFLOP/s).
+// 2048 x 4096 x 11008 took 308 us; 142 us like this).
 //
 // s q has more bits than a 16-bit number. Plain calls round it once, which with the rounding of the output makes 1.4 times
 // (fp16: 1.25 times) the error of the latter. Behind the gate two such products would meet and make it 1.7 times, so
 // gated calls take both parts: CTA 0 makes the rounded weights and CTA 1 what the rounding left, which is exact, for the
 // same 64 rows of both matrices; their products lie in neighbouring accumulator columns and are added in the epilogue.
-// That is twice the tensor work (333 tokens, 4096 x 14336: TIME1 instead of 114 us) and no error beyond fp32 sums.
+// That is twice the tensor work (333 tokens, 4096 x 14336 twice: 190 us instead of 114) and no error beyond fp32 sums.
+//
+// Beyond 128 tokens both are bound by the tensor pipe: 2048 x 4096 x 11008 142 us (1300 TFLOP/s), 4096 x 4096 x 11008
+// 285 us; gated, 4096 -> 14336, 2048 tokens 705 us and 8192 tokens 3.04 ms (1270 TFLOP/s, half of them the rest's).
+// The kernel for 17 to 128 tokens is described below. It pays up to 128: at 65 to 96 tokens 31 us against 34 here with
+// 11008 x 4096, 30 against 32 with 4096 x 4096, 48 against 99 with 4096 x 14336, gated 67 against 115; at 128 tokens 34
+// on both sides, 56 against 100 and 79 against 117.
 #include <algorithm>
 #include <type_traits>
 
@@ -446,14 +452,17 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 // that all SMs have the same number; rows beyond it are stale shared memory in accumulator lanes of their own, not stored.
 // A tensor instruction of so few columns takes 75 clocks however few there are, so a tile costs 600 clocks a block of 128
 // inputs; where 128-row tiles leave SMs free, a cluster of CTAs divides a tile's inputs, and sums its parts through
-// distributed shared memory, in rank order (4096 x 14336, 64 tokens: 61 us without, 30 with).
+// distributed shared memory, in rank order (64 tokens, 4096 x 14336: 89 us without, 33 with; 4096 x 4096: 45 and 20).
 //
 // With so few columns there is time to keep the sums exact: the operand holds the integers, every group of inputs has
 // accumulator columns of its own (a ring of four or eight), and eight warps multiply them by the scale of their lane's
 // row and add them up in registers, in fp32. Nothing is rounded before the result.
 //
+// 64 tokens, cold weights: 11008 x 4096 23 us, 4096 x 14336 33 us, gated 14336 x 4096 twice 49 us (floors 4, 5 and 9): the
+// conversion of the weights and the per-block work of the issuers and sums share the time, not the memory.
+//
 // Waiting for three barriers and issuing eight tensor instructions, one after the other, takes a thread twice the time of
-// the instructions, so two threads issue, one every other block. Rings have even numbers of stages: a barrier's parity
+// the instructions, so two threads issue, one every other block (64 tokens, 11008 x 4096: 31 us with one, 23 with two). Rings have even numbers of stages: a barrier's parity
 // tells a lap from its neighbours only, so whoever waits on one has to see every lap of it.
 struct TokenBars {
     uint64_t *full_w, *empty_w;   // [kTokenRing]: the stage's weight warps; committed by the MMA thread

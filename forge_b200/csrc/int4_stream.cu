@@ -17,6 +17,10 @@
 // 128-input block holds 8 inputs of each of the block's four 32-input runs, so one instruction multiplies inputs of one run
 // only.
 //
+// Cold weights: 11008 x 4096 fp16, groups of 128, 9.7 us at 1 token and 10.6 at 8 (22.5 MB: 2.4 TB/s; 3.6 us at the copy
+// rate, an empty launch 2); 4096 x 14336 bf16, groups of 64, 17 and 18 us; gated 14336 x 4096 twice 22 and 24 us (60.6
+// MB: 2.8 TB/s). 16 tokens need two products a fragment: 17 us for the first.
+//
 // The order of the sums is fixed (blocks of a warp, warps of a CTA): results do not change from run to run. Rows past N
 // and tokens past M are computed on the last one's addresses and not stored.
 #include <algorithm>

@@ -151,6 +151,83 @@ def test_several_passes_over_the_rows(M, K, N, group):
     R.close_rounded(h, *R.gate_of(linear_bound(x, w, s, None, group, True), linear_bound(x, w.flip(0), s, None, group, True)))
 
 
+EDGES = [(16, 8, 1), (17, 8, 1), (17, 64, 129), (32, 4096, 40), (33, 136, 1), (40, 8200, 130), (64, 14336, 72), (64, 264, 300),
+         (65, 4104, 129), (65, 8, 24), (96, 520, 1000), (128, 2056, 40), (128, 128, 257), (129, 8, 1), (129, 8208, 65), (200, 264, 7),
+         (256, 136, 513), (257, 1024, 136)]
+
+
+@pytest.mark.parametrize("dtype,group", [("fp16", 32), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("M,K,N", EDGES)
+def test_both_sides_of_every_choice(M, K, N, dtype, group):
+    """16 | 17, 64 | 65 and 128 | 129 tokens, inputs that are divided over a cluster, tiles with one row or one output."""
+    g = torch.Generator().manual_seed(M + 3 * K + 5 * N + group)
+    x = torch.randn(M, K, generator=g).to(TYPES[dtype]).to(DEV)
+    (wg, sg), (wu, su) = _weight(N, K, group, g), _weight(N, K, group, g)
+    bias = torch.randn(N, generator=g).to(TYPES[dtype]).to(DEV)
+    y = C.int4_linear(x, wg, sg, bias, group)
+    h = C.int4_gated_linear(x, wg, wu, sg, su, bias, None, group)
+    _ok()
+    R.close_rounded(y, *linear_bound(x, wg, sg, bias, group), "linear")
+    R.close_rounded(h, *R.gate_of(linear_bound(x, wg, sg, bias, group, True), linear_bound(x, wu, su, None, group, True)), "gated")
+
+
+def test_several_streams_at_once():
+    """Kernels of every kind side by side, none of which keeps anything that another one writes."""
+    g = torch.Generator().manual_seed(11)
+    w, s = _weight(1100, 2056, 64, g)
+    xs = [torch.randn(M, 2056, generator=g).half().to(DEV) for M in (1, 12, 40, 100, 300)]
+    run = lambda x: (C.int4_linear(x, w, s, None, 64), C.int4_gated_linear(x, w, w, s, s, None, None, 64))  # noqa: E731
+    want = [run(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for k in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                n = (i + k) % len(xs)
+                got.append((n, run(xs[n])))
+    _ok()
+    for n, (y, h) in got:
+        assert torch.equal(y, want[n][0]) and torch.equal(h, want[n][1])
+
+
+_FIRST_CALL_CAPTURED = """
+import torch
+from forge_b200 import _forge_C as C
+from forge_b200.nn import quantize_weight_int4
+dev = torch.device("cuda:0")
+g = torch.Generator().manual_seed(0)
+w, s = (t.to(dev) for t in quantize_weight_int4(torch.randn(48, 136, generator=g) * 0.1, 64))
+W = torch.randn(48, 136, generator=g).half().to(dev) * 0.1
+xs = [torch.randn(M, 136, generator=g).half().to(dev) for M in (1, 40, 100, 200)]
+dh = torch.ones(200, 48, device=dev).half()
+
+def run():
+    out = []
+    for x in xs:
+        out += [C.int4_linear(x, w, s, None, 64), C.int4_gated_linear(x, w, w, s, s, None, None, 64), C.gated_linear(x, W, W)]
+    h, gate, up = C.gated_linear(xs[-1], W, W, save=True)
+    return out + [h, *C.gated_linear_backward(dh, xs[-1], W, W, gate, up)]
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run())) and C.device_status() == 0
+"""
+
+
+def test_a_first_call_may_be_captured():
+    """In a process of its own, where no kernel has been loaded or set up."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("M", [1, 8, 40])
 def test_repeated_calls_give_the_same_bits(M):
     g = torch.Generator().manual_seed(M)

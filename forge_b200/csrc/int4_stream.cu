@@ -34,7 +34,6 @@ namespace fb200 {
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kRing = 6;              // KB of a warp's weights under way: 6 * 24 warps, and room for activations in L1
 constexpr int kTokStride = 20;        // floats per token of a partial sum: 16 rows + 4, conflict-free fragment writes
 
@@ -82,9 +81,9 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// UNITS: blocks of 16 rows of a warp. NT: blocks of 8 tokens.
-template <typename T, int G, bool GATED, int UNITS, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+// UNITS: blocks of 16 rows of a CTA. NT: blocks of 8 tokens.
+template <typename T, int G, bool GATED, int UNITS, int WARPS, int NT>
+__global__ void __launch_bounds__(WARPS * 32, (NT == 1 ? 24 : 16) / WARPS)
 int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
                    const __half* __restrict__ s0, const __half* __restrict__ s1, const T* __restrict__ b0,
                    const T* __restrict__ b1, T* __restrict__ out, int M, int K, int N, int rows) {
@@ -92,14 +91,13 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
     constexpr int PER = 128 / G, FLUSH = G / 32;   // groups of a block; runs of a group
     constexpr int kDepth = kRing / UNITS;          // blocks under way
     constexpr int RED_UNIT = NT * 8 * kTokStride;
-    constexpr int RING = kWarps * kDepth * UNITS * 1024, RED = kWarps * UNITS * RED_UNIT * 4;
-    __shared__ __align__(16) uint8_t smem[RING > RED ? RING : RED];
+    extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * rows;
     const int m0 = blockIdx.y * (NT * 8);
     const int blocks = (K + 127) / 128;
-    const int mine = warp < blocks ? (blocks - warp + kWarps - 1) / kWarps : 0;
-    const bool ragged = K % 128 != 0 && mine > 0 && warp + (mine - 1) * kWarps == blocks - 1;
+    const int mine = warp < blocks ? (blocks - warp + WARPS - 1) / WARPS : 0;
+    const bool ragged = K % 128 != 0 && mine > 0 && warp + (mine - 1) * WARPS == blocks - 1;
 
     const uint8_t* wp[UNITS][2];
 #pragma unroll
@@ -117,7 +115,7 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 cp_async16(ring + in_stage * (UNITS * 1024) + u * 1024 + r * 512, wp[u][r]);
-                wp[u][r] += kWarps * 64;
+                wp[u][r] += WARPS * 64;
             }
         in_stage = in_stage + 1 == kDepth ? 0 : in_stage + 1;
     };
@@ -159,10 +157,10 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
                 if (WHOLE || block * 128 + j * 32 + t * 8 < K) xv[j][n] = __ldg(reinterpret_cast<const uint4*>(xp[n] + j * 32));
             }
 #pragma unroll
-        for (int n = 0; n < NT; n++) xp[n] += kWarps * 128;
+        for (int n = 0; n < NT; n++) xp[n] += WARPS * 128;
 #pragma unroll
         for (int k = 0; k < PER; k++) sv[k] = sn[k];
-        load_scales(min(block + kWarps, blocks - 1), sn);
+        load_scales(min(block + WARPS, blocks - 1), sn);
         cp_wait<kDepth - 1>();
         float off[PER][NT][2];   // minus the offset's share of the lane's two tokens, per group
 #pragma unroll
@@ -209,7 +207,7 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
                 }
             }
         }
-        block += kWarps;
+        block += WARPS;
         stage = stage + 1 == kDepth ? 0 : stage + 1;
     };
     const int whole = mine - ragged;
@@ -235,7 +233,7 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
             p[kTokStride + 8] = acc[u][n][3];
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < (GATED ? 1 : UNITS) * NT * 128; i += kWarps * 32) {
+    for (int i = threadIdx.x; i < (GATED ? 1 : UNITS) * NT * 128; i += WARPS * 32) {
         const int row = i % 16, u = GATED ? 0 : i / 16 % UNITS, tok = i / 16 / (GATED ? 1 : UNITS);
         const int m = m0 + tok, n = n0 + u * 16 + row;
         if (m >= M || n >= N || u * 16 + row >= rows) continue;
@@ -243,7 +241,7 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
             const float* p = red + unit * RED_UNIT + tok * kTokStride + row;
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; w++) v += p[w * (UNITS * RED_UNIT)];
+            for (int w = 0; w < WARPS; w++) v += p[w * (UNITS * RED_UNIT)];
             return v * F::kFactor;
         };
         float v = sum(u) + (b0 != nullptr ? to_float(b0[n]) : 0.f);
@@ -252,34 +250,53 @@ int4_stream_kernel(const T* __restrict__ x, const uint8_t* __restrict__ w0, cons
     }
 }
 
-template <typename T, int G, bool GATED, int UNITS, int NT>
+template <typename T, int G, bool GATED, int UNITS, int WARPS, int NT>
 int launch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
-           const void* b1, void* out, int M, int K, int N, cudaStream_t stream) {
-    // output channels of a CTA: as many as a warp can hold, or, where every SM gets at most the three CTAs that it runs at
-    // a time, so many that all SMs get the same number of CTAs (4096 channels: 14 of 16, two CTAs an SM)
-    int rows = GATED ? 16 : 16 * UNITS;
-    const int per_sm = (int)std::min<long long>(4, ((long long)N + (long long)rows * sm_count() - 1) / ((long long)rows * sm_count()));
-    if (per_sm <= 3) rows = (N + per_sm * sm_count() - 1) / (per_sm * sm_count());
+           const void* b1, void* out, int M, int K, int N, int rows, cudaStream_t stream) {
+    static bool ready[64] = {};
+    auto kern = int4_stream_kernel<T, G, GATED, UNITS, WARPS, NT>;
+    constexpr int kSmem = std::max(WARPS * kRing * 1024, WARPS * UNITS * NT * 8 * kTokStride * 4);
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!ready[dev & 63]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+            return kLaunchFailed;
+        ready[dev & 63] = true;
+    }
     const dim3 grid((unsigned)(((long long)N + rows - 1) / rows), (M + NT * 8 - 1) / (NT * 8), 1);
     if (grid.y > 65535) return kTooLarge;
-    int4_stream_kernel<T, G, GATED, UNITS, NT><<<grid, kWarps * 32, 0, stream>>>(
-        static_cast<const T*>(x), w0, w1, s0, s1, static_cast<const T*>(b0), static_cast<const T*>(b1), static_cast<T*>(out),
-        M, K, N, rows);
+    kern<<<grid, WARPS * 32, kSmem, stream>>>(static_cast<const T*>(x), w0, w1, s0, s1, static_cast<const T*>(b0),
+                                              static_cast<const T*>(b1), static_cast<T*>(out), M, K, N, rows);
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
+}
+
+template <typename T, int G, bool GATED>
+int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
+             const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
+    // Output channels of a CTA: as many as a warp can hold, or, where that makes up to three CTAs for each SM, so many that
+    // all SMs have the same number. The warps that an SM runs at a time (24; 16 with more than 8 tokens) are divided over
+    // them: 4096 x 14336 14 us with 24 warps on 28 channels, 17 with 8 on 14 twice; 8192 x 8192 12 us with 12 warps on 28
+    // channels twice, 17 with 8 on 14 four times.
+    const int most = GATED ? 16 : 32, sms = sm_count();
+    const long long per_sm = ((long long)N + (long long)most * sms - 1) / ((long long)most * sms);
+    const int rows = per_sm <= 3 ? (int)((N + per_sm * sms - 1) / (per_sm * sms)) : most;
+    if (!GATED && rows <= 16)   // 2048 x 2048: 4.2 us with fragments for 32
+        return M <= 8 ? launch<T, G, false, 1, 24, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st)
+                      : launch<T, G, false, 1, 16, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
+    if (M <= 8) {
+        if (per_sm == 1) return launch<T, G, GATED, 2, 24, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
+        if (per_sm == 2) return launch<T, G, GATED, 2, 12, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
+        return launch<T, G, GATED, 2, 8, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
+    }
+    if (per_sm == 1) return launch<T, G, GATED, 2, 16, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
+    return launch<T, G, GATED, 2, 8, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
 }
 
 template <typename T, int G>
 int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
              const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
-    if (w1 != nullptr)
-        return M <= 8 ? launch<T, G, true, 2, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                      : launch<T, G, true, 2, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
-    // 32 rows a warp share the activations and the offset; 16 where there are too few CTAs otherwise
-    if (N > 32 * 2 * sm_count())
-        return M <= 8 ? launch<T, G, false, 2, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                      : launch<T, G, false, 2, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
-    return M <= 8 ? launch<T, G, false, 1, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
-                  : launch<T, G, false, 1, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
+    return w1 != nullptr ? dispatch<T, G, true>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                         : dispatch<T, G, false>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
 }
 
 }  // namespace

@@ -10,16 +10,19 @@
 //     and the sums are fp32: nothing is rounded before the result, but a token with an infinite activation comes out as
 //     NaN.
 //   - The products are tensor-core fragments, whose cost does not grow with the tokens up to 8 per instruction.
-//   - A warp owns 16 or 32 output channels of the call (gated: 16 of each matrix) and every eighth block of 128 inputs. A
-//     lane copies exactly the bytes that it later reads as its fragment (cp.async, a ring of its own), so
-//     warps run without barriers, three CTAs of eight on an SM, up to the sum over a CTA's warps at the end.
+//   - A CTA owns up to 32 output channels of the call (gated: 16 of each matrix) and its warps divide the blocks of 128
+//     inputs. A lane copies exactly the bytes that it later reads as its fragment (cp.async, a ring of its own), so warps
+//     run without barriers, 24 on an SM, up to the sum over a CTA's warps at the end. Activations are read through L1:
+//     copied into the ring as well they cost a third of the weights' stages, and calls with 8 and 16 tokens 5 to 20 %.
 // The weight layout (forge_prepare_weight_int4) makes this possible for every group size: a lane's 16-byte load of a
 // 128-input block holds 8 inputs of each of the block's four 32-input runs, so one instruction multiplies inputs of one run
 // only.
 //
-// Cold weights: 11008 x 4096 fp16, groups of 128, 9.7 us at 1 token and 10.6 at 8 (22.5 MB: 2.4 TB/s; 3.6 us at the copy
-// rate, an empty launch 2); 4096 x 14336 bf16, groups of 64, 17 and 18 us; gated 14336 x 4096 twice 22 and 24 us (60.6
-// MB: 2.8 TB/s). 16 tokens need two products a fragment: 17 us for the first.
+// Cold weights: 11008 x 4096 fp16, groups of 128, 9.7 us at 1 token and 10.6 at 8 (22.9 MB: 2.4 TB/s; 3.5 us at the copy
+// rate, an empty launch 2); 4096 x 14336 bf16, groups of 64, 14 and 15 us; 8192 x 8192 12 and 12.6; 28672 x 8192 32 us (3.7
+// TB/s); gated 14336 x 4096 twice 22 and 24 us (60.6 MB: 2.8 TB/s). 4096 x 14336: half of the issue slots are used and a
+// fifth of the memory's rate; what is left is latency, of the activations from L2 and of few blocks for each warp. 16
+// tokens need two products a fragment and the registers of 16 warps an SM: 17 us for the first.
 //
 // The order of the sums is fixed (blocks of a warp, warps of a CTA): results do not change from run to run. Rows past N
 // and tokens past M are computed on the last one's addresses and not stored.
@@ -34,7 +37,7 @@ namespace fb200 {
 
 namespace {
 
-constexpr int kRing = 6;              // KB of a warp's weights under way: 6 * 24 warps, and room for activations in L1
+constexpr int kRing = 6;              // KB of a warp's weights under way: 6 * 24 warps, and room for activations in L1 (8: 5 % slower)
 constexpr int kTokStride = 20;        // floats per token of a partial sum: 16 rows + 4, conflict-free fragment writes
 
 // Word of 8 four-bit weights (weight 2i in nibble i, weight 2i + 1 in nibble i + 4, stored as the integer + 8) -> four
@@ -280,7 +283,7 @@ int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* 
     const int most = GATED ? 16 : 32, sms = sm_count();
     const long long per_sm = ((long long)N + (long long)most * sms - 1) / ((long long)most * sms);
     const int rows = per_sm <= 3 ? (int)((N + per_sm * sms - 1) / (per_sm * sms)) : most;
-    if (!GATED && rows <= 16)   // 2048 x 2048: 4.2 us with fragments for 32
+    if (!GATED && rows <= 16)   // 2048 x 2048: 3.3 us, 4.2 with fragments for 32
         return M <= 8 ? launch<T, G, false, 1, 24, 1>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st)
                       : launch<T, G, false, 1, 16, 2>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, rows, st);
     if (M <= 8) {

@@ -331,7 +331,8 @@ def gated_linear(x, Wg, Wu, bg=None, bu=None, save=False):
     h = x.new_empty((M, N))
     g = u = None
     if save:
-        g, u = x.new_empty((M, N), dtype=_f32), x.new_empty((M, N), dtype=_f32)
+        g = x.new_empty((M, N), dtype=_f32)
+        u = torch.empty_like(g)
     _run(x, "forge_gated_linear", x.data_ptr(), Wg.data_ptr(), Wu.data_ptr(), _ptr(bg), _ptr(bu), h.data_ptr(), _ptr(g),
          _ptr(u), M, K, N, dtype)
     return (h, g, u) if save else h
@@ -346,10 +347,13 @@ def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=
     if N % 8 != 0 or N > _MAX_SIZE:
         raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, at most {_MAX_SIZE}, got {N}")
     # without tokens the library writes nothing, and the gradients of the weights are zero
-    new = torch.zeros if M == 0 else torch.empty
-    dx = new((M, K), dtype=x.dtype, device=x.device) if need_x else None
-    dWg, dWu = (new((N, K), dtype=x.dtype, device=x.device) if need_w else None for _ in range(2))
-    dbg, dbu = (new((N,), dtype=x.dtype, device=x.device) if need_b else None for _ in range(2))
+    like = torch.zeros_like if M == 0 else torch.empty_like
+    dx = like(x) if need_x else None
+    dWg, dWu = (like(Wg), like(Wu)) if need_w else (None, None)
+    dbg = dbu = None
+    if need_b:
+        dbg = x.new_zeros((N,)) if M == 0 else x.new_empty((N,))
+        dbu = like(dbg)
     dh, x, Wg, Wu = _aligned(dh), _aligned(x), _aligned(Wg), _aligned(Wu)
     g, u = _aligned(g), _aligned(u)
     size = _lib.load().forge_gated_linear_backward_workspace_bytes(M, N)

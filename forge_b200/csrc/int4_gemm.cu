@@ -18,8 +18,10 @@
 // same 64 rows of both matrices; their products lie in neighbouring accumulator columns and are added in the epilogue.
 // That is twice the tensor work (333 tokens, 4096 x 14336 twice: 190 us instead of 114) and no error beyond fp32 sums.
 //
-// Beyond 128 tokens both are bound by the tensor pipe: 2048 x 4096 x 11008 142 us (1300 TFLOP/s), 4096 x 4096 x 11008
-// 285 us; gated, 4096 -> 14336, 2048 tokens 705 us and 8192 tokens 3.04 ms (1270 TFLOP/s, half of them the rest's).
+// Beyond 128 tokens: 2048 x 4096 x 11008 142 us (1300 TFLOP/s, tensor pipe 71 % busy), 4096 x 4096 x 11008 285 us; gated,
+// 4096 -> 14336, 2048 tokens 705 us (74 %) and 8192 tokens 2.8-3.0 ms (1300 TFLOP/s, half of them the rest's). A block takes
+// 0.88 us where its tensor instructions take 0.55: a stage is refilled once they are done with it, and 192 KB are three.
+// Weights made in registers ahead of the stage do not help (156 us: the registers spill).
 // The kernel for 17 to 128 tokens is described below. It pays up to 128: at 65 to 96 tokens 31 us against 34 here with
 // 11008 x 4096, 30 against 32 with 4096 x 4096, 48 against 99 with 4096 x 14336, gated 67 against 115; at 128 tokens 34
 // on both sides, 56 against 100 and 79 against 117.
@@ -912,8 +914,8 @@ int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* 
         return gated ? launch_tokens<T, G, true, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
                      : launch_tokens<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     if (gated) return launch<T, G, true, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
-    // 128 weight rows a tile take 0.6 of the time of 256 (tensor instructions of 128 columns run at their floor of 86
-    // clocks): where even those leave pairs without a tile
+    // A round of tiles of 128 weight rows takes 0.9 of the time of 256: worth it where even those fit into one round
+    // (512 x 14336 x 4096: 88 against 94 us), not for shorter but more rounds (512 x 4096 x 11008: 81 against 59).
     const long long wide = ((long long)M + 255) / 256 * (((long long)N + 255) / 256);
     return 2 * wide <= sm_count() / 2 ? launch<T, G, false, 128>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
                                       : launch<T, G, false, 256>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);

@@ -458,7 +458,8 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 //
 // With so few columns there is time to keep the sums exact: the operand holds the integers, every group of inputs has
 // accumulator columns of its own (a ring of four or eight), and eight warps multiply them by the scale of their lane's
-// row and add them up in registers, in fp32. Nothing is rounded before the result.
+// row and add them up in registers, in fp32. Nothing is rounded before the result. A block's groups are waited for and
+// released together (11008 x 4096, 64 tokens, groups of 32: 51 us one by one, 39 like this).
 //
 // 64 tokens, cold weights: 11008 x 4096 23 us, 4096 x 14336 33 us, gated 14336 x 4096 twice 49 us (floors 4, 5 and 9): the
 // conversion of the weights and the per-block work of the issuers and sums share the time, not the memory.
@@ -469,7 +470,7 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 struct TokenBars {
     uint64_t *full_w, *empty_w;   // [kTokenRing]: the stage's weight warps; committed by the MMA thread
     uint64_t *full_x, *empty_x;   // [kMaxRingX]
-    uint64_t *tmem_full, *tmem_empty;   // [kMaxAccs]
+    uint64_t *tmem_full, *tmem_empty;   // [kMaxAccs], one for each set of accumulators
     uint32_t* tmem_slot;
     volatile int* abort_flag;
 };
@@ -559,7 +560,9 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *bars.tmem_slot;
+    // Accumulators change hands in sets: a block's groups, or as many of them as leave another set to work on
     constexpr int accs = 512 / MAX_COLS, acc_cols = MAX_COLS;
+    constexpr int SET = PER <= accs / 2 ? PER : accs / 2, SETS = accs / SET, BLOCK_SETS = PER / SET;
 
     if (warp_id == 0) {
         // ------------------------------------------------------------------ activations (TMA)
@@ -604,21 +607,22 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                 const uint64_t da = make_desc_sw128(smem_u32(smem + stage * 2 * kSlab));
                 const uint64_t db = make_desc_sw128(smem_u32(smem_x + stage_x * 2 * slab_x));
 #pragma unroll
-                for (int k = 0; k < PER; k++) {
-                    const int a = i * PER + k, acc = a & (accs - 1);
-                    if (!mbar_wait(&bars.tmem_empty[acc], ((a / accs) & 1) ^ 1, bars.abort_flag)) {
+                for (int h = 0; h < BLOCK_SETS; h++) {
+                    const int a = i * BLOCK_SETS + h, set = a & (SETS - 1);
+                    if (!mbar_wait(&bars.tmem_empty[set], ((a / SETS) & 1) ^ 1, bars.abort_flag)) {
                         atomicExch(status, 852);
                         ok = false;
                         break;
                     }
                     tc_fence_after();
 #pragma unroll
-                    for (int e = 0; e < G / 16; e++) {
-                        const int step = k * (G / 16) + e;   // of the block's eight
-                        umma_f16(tmem_base + acc * acc_cols, da + (step / 4) * (kSlab >> 4) + 2 * (step % 4),
-                                 db + (step / 4) * (slab_x >> 4) + 2 * (step % 4), idesc, e != 0 ? 1u : 0u);
+                    for (int e = 0; e < SET * (G / 16); e++) {
+                        const int step = h * SET * (G / 16) + e;   // of the block's eight
+                        umma_f16(tmem_base + (set * SET + e / (G / 16)) * acc_cols,
+                                 da + (step / 4) * (kSlab >> 4) + 2 * (step % 4),
+                                 db + (step / 4) * (slab_x >> 4) + 2 * (step % 4), idesc, e % (G / 16) != 0 ? 1u : 0u);
                     }
-                    tc_commit(&bars.tmem_full[acc]);
+                    tc_commit(&bars.tmem_full[set]);
                 }
                 tc_commit(&bars.empty_w[stage]);
                 tc_commit(&bars.empty_x[stage_x]);
@@ -690,8 +694,8 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
         const int q = warp_id & 3, half = (warp_id - kFirstSum) / 4;
         const int width = cols / 2, col0 = half * width;   // a multiple of 16, at most 64
         float* swap = reinterpret_cast<float*>(smem_swap);
-        int acc = 0;
-        uint32_t phase_acc = 0;
+        int set = 0;
+        uint32_t phase_set = 0;
         bool ok = true;
         for (int t = first_tile; t < num_tiles; t += tile_step) {
             const int r = GATED ? (q % 2) * 32 + lane : q * 32 + lane;
@@ -718,36 +722,39 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             for (int i = 0; i < SUMS; i++) sum[i] = 0.f;
             auto add = [&](unsigned short (&scales)[PER]) {   // the products of the next block
 #pragma unroll
-                for (int k = 0; k < PER; k++) {
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[acc], phase_acc, bars.abort_flag));
+                for (int h = 0; h < BLOCK_SETS; h++) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.tmem_full[set], phase_set, bars.abort_flag));
                     if (!ok) return;
                     tc_fence_after();
-                    const float s = __half2float(__ushort_as_half(scales[k]));
-                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * acc_cols + col0;
+                    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + set * SET * acc_cols + col0;
                     constexpr int CHUNK = SUMS > 32 ? 16 : 32;   // columns at a time, as the registers allow
 #pragma unroll
-                    for (int c = 0; c < SUMS / CHUNK; c++) {
-                        // columns past `width` may hold anything: theirs are sums that nobody takes
-                        uint32_t v[CHUNK];
-                        if (c * CHUNK < width) {
-                            if constexpr (CHUNK == 16) tmem_ld_32x32b_x16(taddr + c * CHUNK, v);
-                            else tmem_ld_32x32b_x32(taddr + c * CHUNK, v);
-                            tmem_ld_wait();
-                        }
-                        if (c == SUMS / CHUNK - 1) {   // all of it is in registers
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&bars.tmem_empty[acc]);
-                        }
-                        if (c * CHUNK < width) {
+                    for (int k = 0; k < SET; k++) {
+                        const float s = __half2float(__ushort_as_half(scales[h * SET + k]));
 #pragma unroll
-                            for (int e = 0; e < CHUNK; e++)
-                                sum[c * CHUNK + e] = fmaf(__uint_as_float(v[e]), s, sum[c * CHUNK + e]);
+                        for (int c = 0; c < SUMS / CHUNK; c++) {
+                            // columns past `width` may hold anything: theirs are sums that nobody takes
+                            uint32_t v[CHUNK];
+                            if (c * CHUNK < width) {
+                                if constexpr (CHUNK == 16) tmem_ld_32x32b_x16(taddr + k * acc_cols + c * CHUNK, v);
+                                else tmem_ld_32x32b_x32(taddr + k * acc_cols + c * CHUNK, v);
+                                tmem_ld_wait();
+                            }
+                            if (k == SET - 1 && c == SUMS / CHUNK - 1) {   // all of the set is in registers
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&bars.tmem_empty[set]);
+                            }
+                            if (c * CHUNK < width) {
+#pragma unroll
+                                for (int e = 0; e < CHUNK; e++)
+                                    sum[c * CHUNK + e] = fmaf(__uint_as_float(v[e]), s, sum[c * CHUNK + e]);
+                            }
                         }
                     }
-                    if (++acc == accs) {
-                        acc = 0;
-                        phase_acc ^= 1;
+                    if (++set == SETS) {
+                        set = 0;
+                        phase_set ^= 1;
                     }
                 }
             };

@@ -507,7 +507,7 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uin
         : "memory");
 }
 
-// MAX_COLS: 64 or 128
+// MAX_COLS: 32, 64 or 128
 template <typename T, int G, bool GATED, int MAX_COLS>
 __global__ void __launch_bounds__(kTokenThreads, 1)
 int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __restrict__ w0, const uint8_t* __restrict__ w1,
@@ -561,7 +561,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
     tc_fence_after();
     const uint32_t tmem_base = *bars.tmem_slot;
     // Accumulators change hands in sets: a block's groups, or as many of them as leave another set to work on
-    constexpr int accs = 512 / MAX_COLS, acc_cols = MAX_COLS;
+    constexpr int accs = MAX_COLS > 64 ? 4 : 8, acc_cols = MAX_COLS;
     constexpr int SET = PER <= accs / 2 ? PER : accs / 2, SETS = accs / SET, BLOCK_SETS = PER / SET;
 
     if (warp_id == 0) {
@@ -727,7 +727,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     if (!ok) return;
                     tc_fence_after();
                     const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + set * SET * acc_cols + col0;
-                    constexpr int CHUNK = SUMS > 32 ? 16 : 32;   // columns at a time, as the registers allow
+                    constexpr int CHUNK = SUMS == 32 ? 32 : 16;   // columns at a time, as the registers allow
 #pragma unroll
                     for (int k = 0; k < SET; k++) {
                         const float s = __half2float(__ushort_as_half(scales[h * SET + k]));
@@ -914,6 +914,9 @@ template <typename T, int G>
 int dispatch(const void* x, const uint8_t* w0, const uint8_t* w1, const __half* s0, const __half* s1, const void* b0,
              const void* b1, void* out, int M, int K, int N, cudaStream_t st) {
     const bool gated = w1 != nullptr;
+    if (M <= 32)
+        return gated ? launch_tokens<T, G, true, 32>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
+                     : launch_tokens<T, G, false, 32>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);
     if (M <= 64)
         return gated ? launch_tokens<T, G, true, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st)
                      : launch_tokens<T, G, false, 64>(x, w0, w1, s0, s1, b0, b1, out, M, K, N, st);

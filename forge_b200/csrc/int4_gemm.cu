@@ -707,7 +707,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
             const int groups = (K + G - 1) / G;
             // Scales of AHEAD blocks, and of the AHEAD behind them under way: a block takes less time than a load, and loads
             // between the uses of earlier ones would make those wait for them.
-            constexpr int AHEAD = (MAX_COLS > 64 ? 4 : 8) / PER;   // as the registers allow
+            constexpr int AHEAD = (MAX_COLS > 32 ? 4 : 8) / PER;   // as the registers allow
             unsigned short now[AHEAD][PER], next[AHEAD][PER];
             auto load = [&](int blk) {
 #pragma unroll

@@ -153,7 +153,7 @@ def test_several_passes_over_the_rows(M, K, N, group):
 
 EDGES = [(16, 8, 1), (17, 8, 1), (17, 64, 129), (32, 4096, 40), (33, 136, 1), (40, 8200, 130), (64, 14336, 72), (64, 264, 300),
          (65, 4104, 129), (65, 8, 24), (96, 520, 1000), (128, 2056, 40), (128, 128, 257), (129, 8, 1), (129, 8208, 65), (200, 264, 7),
-         (256, 136, 513), (257, 1024, 136)]
+         (256, 136, 513), (257, 1024, 136), (100, 2056, 9500), (70, 6152, 4100)]
 
 
 @pytest.mark.parametrize("dtype,group", [("fp16", 32), ("bf16", 64), ("fp16", 128)])

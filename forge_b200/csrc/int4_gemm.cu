@@ -22,9 +22,9 @@
 // 4096 -> 14336, 2048 tokens 705 us (74 %) and 8192 tokens 2.8-3.0 ms (1300 TFLOP/s, half of them the rest's). A block takes
 // 0.88 us where its tensor instructions take 0.55: a stage is refilled once they are done with it, and 192 KB are three.
 // Weights made in registers ahead of the stage do not help (156 us: the registers spill).
-// The kernel for 17 to 128 tokens is described below. It pays up to 128: at 65 to 96 tokens 31 us against 34 here with
-// 11008 x 4096, 30 against 32 with 4096 x 4096, 48 against 99 with 4096 x 14336, gated 67 against 115; at 128 tokens 34
-// on both sides, 56 against 100 and 79 against 117.
+// The kernel for 17 to 128 tokens is described below. It pays up to 128, apart from its sums: at 65 to 96 tokens 31 us
+// against 34 here with 11008 x 4096 and groups of 128 (with groups of 32 50), 45 against 95 with 4096 x 14336, gated 67
+// against 115; at 128 tokens 34 on both sides, 48 against 95 and 78 against 117.
 #include <algorithm>
 #include <type_traits>
 
@@ -454,19 +454,21 @@ int4_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant
 // that all SMs have the same number; rows beyond it are stale shared memory in accumulator lanes of their own, not stored.
 // A tensor instruction of so few columns takes 75 clocks however few there are, so a tile costs 600 clocks a block of 128
 // inputs; where 128-row tiles leave SMs free, a cluster of CTAs divides a tile's inputs, and sums its parts through
-// distributed shared memory, in rank order (64 tokens, 4096 x 14336: 89 us without, 33 with; 4096 x 4096: 45 and 20).
+// distributed shared memory, in rank order (64 tokens, 4096 x 14336: 61 us without, 25 with; 4096 x 4096: 21 and 13).
 //
 // With so few columns there is time to keep the sums exact: the operand holds the integers, every group of inputs has
 // accumulator columns of its own (a ring of four or eight), and eight warps multiply them by the scale of their lane's
 // row and add them up in registers, in fp32. Nothing is rounded before the result. A block's groups are waited for and
-// released together (11008 x 4096, 64 tokens, groups of 32: 51 us one by one, 39 like this).
+// released together; what sums cost otherwise is registers: 32 columns where there are no more tokens, and as few scales ahead
+// as hide a load (11008 x 4096, groups of 32, 64 tokens: 51 us without these, 28 with; 32 tokens: 51 and 22).
 //
-// 64 tokens, cold weights: 11008 x 4096 23 us, 4096 x 14336 33 us, gated 14336 x 4096 twice 49 us (floors 4, 5 and 9): the
-// conversion of the weights and the per-block work of the issuers and sums share the time, not the memory.
+// 64 tokens, cold weights: 11008 x 4096 22 us, 4096 x 14336 25 us, gated 14336 x 4096 twice 45 us (floors 4, 5 and 9): the
+// conversion of the weights and the per-block work of the issuers and sums take the time, not the memory.
 //
 // Waiting for three barriers and issuing eight tensor instructions, one after the other, takes a thread twice the time of
-// the instructions, so two threads issue, one every other block (64 tokens, 11008 x 4096: 31 us with one, 23 with two). Rings have even numbers of stages: a barrier's parity
-// tells a lap from its neighbours only, so whoever waits on one has to see every lap of it.
+// the instructions, so two threads issue, one every other block (64 tokens, 11008 x 4096: 31 us with one, 22 with two).
+// Rings have even numbers of stages: a barrier's parity tells a lap from its neighbours only, so whoever waits on one has
+// to see every lap of it.
 struct TokenBars {
     uint64_t *full_w, *empty_w;   // [kTokenRing]: the stage's weight warps; committed by the MMA thread
     uint64_t *full_x, *empty_x;   // [kMaxRingX]

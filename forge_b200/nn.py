@@ -237,14 +237,15 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None):
 
     A step can be captured into a CUDA graph. As with every autograd operation, no graph recorded outside the capture may
     then still be alive for the same leaves: its gradient accumulators belong to the stream it was recorded on."""
-    x2 = x.reshape(-1, x.shape[-1]).contiguous()
+    flat = x.dim() == 2   # no reshapes then: each would be a node of its own in the backward pass
+    x2 = (x if flat else x.reshape(-1, x.shape[-1])).contiguous()
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     args = (x2, w_gate, w_up, b_gate, b_up)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         h = _GatedLinearFn.apply(*args)
     else:
         h = _C.gated_linear(*args)
-    return h.reshape(*x.shape[:-1], w_gate.shape[0])
+    return h if flat else h.reshape(*x.shape[:-1], w_gate.shape[0])
 
 
 class GatedLinear(nn.Module):

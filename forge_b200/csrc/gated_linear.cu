@@ -18,7 +18,7 @@
 //
 // 8192 tokens, 4096 -> 14336, bf16: forward 1.20 ms (1600 TFLOP/s, the burst rate of the tensor pipe), with g and u saved
 // 1.31 ms; backward 2.8-3.0 ms, of which the elementwise part takes 265 us and the products the rest (1500 TFLOP/s). 1001
-// tokens, 1032 -> 2744: forward 41 us, backward 103 us, with tens of tiles for 74 pairs; a step through autograd takes
+// tokens, 1032 -> 2744: forward 25 us, backward 64 us, with tens of tiles for 74 pairs; a step through autograd takes
 // 155 us of host time.
 //
 // Precision: the forward keeps g and u in fp32 for the backward - 8 bytes per element, where rounding them to 16 bits

@@ -170,8 +170,11 @@ def _check_weight(module, *weights):
             raise ValueError(f"weight: expected shape {(module.out_features, module.in_features)}, got {tuple(w.shape)}")
 
 
-def _as_16bit_rows(x, dtype):
-    """x as contiguous (rows, features) in fp16 or bf16 (other types are converted to `dtype`), and its leading sizes."""
+def _as_16bit_rows(x, features, dtype):
+    """x as contiguous (rows, features) in fp16 or bf16 (other types are converted to `dtype`), and its leading sizes.
+    The packed weight does not tell the number of inputs, only that of its groups and blocks: it is checked here."""
+    if x.shape[-1:] != (features,):
+        raise ValueError(f"x: expected (..., {features}), got {tuple(x.shape)}")
     if x.dtype not in (torch.float16, torch.bfloat16):
         x = x.to(dtype)
     return x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
@@ -197,7 +200,7 @@ class Int4Linear(nn.Module):
             self.register_parameter("bias", None)
 
     def forward(self, x):
-        x2, lead = _as_16bit_rows(x, self.dtype)
+        x2, lead = _as_16bit_rows(x, self.in_features, self.dtype)
         bias = None if self.bias is None else self.bias.detach().to(x2.dtype)
         y = _C.int4_linear(x2.detach(), self.w_int4, self.w_scale, bias, self.group_size)
         return y.reshape(*lead, self.out_features)
@@ -300,7 +303,7 @@ class Int4GatedLinear(nn.Module):
                 self.register_parameter(f"b_{k}", None)
 
     def forward(self, x):
-        x2, lead = _as_16bit_rows(x, self.dtype)
+        x2, lead = _as_16bit_rows(x, self.in_features, self.dtype)
         bg, bu = (None if b is None else b.detach().to(x2.dtype) for b in (self.b_gate, self.b_up))
         h = _C.int4_gated_linear(x2.detach(), self.w_gate_int4, self.w_up_int4, self.w_gate_scale, self.w_up_scale, bg, bu,
                                  self.group_size)

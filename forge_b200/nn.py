@@ -19,6 +19,7 @@ import math
 import numpy as np
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _forge_C as _C
 
@@ -217,6 +218,12 @@ class Int4Linear(nn.Module):
                 f"bias={self.bias is not None}, group_size={self.group_size}")
 
 
+def _has_tangent(tensors):
+    """Whether forward-mode differentiation is under way and one of `tensors` (or None) carries a tangent."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _GatedLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up):
@@ -235,8 +242,9 @@ class _GatedLinearFn(torch.autograd.Function):
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None):
-    """SiLU(x w_gate^T + b_gate) * (x w_up^T + b_up), differentiable in every argument. x (..., K), weights (N, K), biases
-    (N), all fp16 or all bf16, K and N multiples of 8. In training the two products are kept in fp32.
+    """SiLU(x w_gate^T + b_gate) * (x w_up^T + b_up), differentiable in every argument by backward passes (forward mode
+    raises). x (..., K), weights (N, K), biases (N), all fp16 or all bf16, K and N multiples of 8. In training the two
+    products are kept in fp32.
 
     A step can be captured into a CUDA graph. As with every autograd operation, no graph recorded outside the capture may
     then still be alive for the same leaves: its gradient accumulators belong to the stream it was recorded on."""
@@ -244,7 +252,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None):
     x2 = (x if flat else x.reshape(-1, x.shape[-1])).contiguous()
     w_gate, w_up = w_gate.contiguous(), w_up.contiguous()
     args = (x2, w_gate, w_up, b_gate, b_up)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    # with a tangent `apply` raises, as there is no forward-mode formula; the bare call would drop it
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)) or _has_tangent(args):
         h = _GatedLinearFn.apply(*args)
     else:
         h = _C.gated_linear(*args)

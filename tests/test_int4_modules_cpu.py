@@ -2,24 +2,25 @@
 with the entry points replaced by stand-ins where a call would reach them."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from forge_b200 import _forge_C as C
-from forge_b200.nn import Int4GatedLinear, Int4Linear
+from forge_b200.nn import GatedLinear, Int4GatedLinear, Int4Linear, gated_linear
 
 
 @pytest.fixture
 def entry_points(monkeypatch):
-    """The inference calls answer with zeros of the right shape and remember what they were given."""
+    """The forward calls answer with zeros of the right shape and remember what they were given."""
     calls = []
 
-    def answer(name, outputs):
-        def call(x, *args):
-            calls.append((name, x, args))
-            return x.new_zeros((x.shape[0], outputs(args)))
+    def answer(name):
+        def call(x, w, *args, save=False):
+            calls.append((name, x, w, args))
+            y = x.new_zeros((x.shape[0], w.shape[0]))
+            return (y, y.float(), y.float()) if save else y
         return call
-    monkeypatch.setattr(C, "int4_linear", answer("int4_linear", lambda a: a[0].shape[0]))
-    monkeypatch.setattr(C, "int4_gated_linear", answer("int4_gated_linear", lambda a: a[0].shape[0]))
-    monkeypatch.setattr(C, "gated_linear", answer("gated_linear", lambda a: a[0].shape[0]))
+    for name in ("int4_linear", "int4_gated_linear", "gated_linear"):
+        monkeypatch.setattr(C, name, answer(name))
     return calls
 
 
@@ -39,3 +40,28 @@ def test_inputs_of_another_width_are_refused(entry_points, make, group, features
     with pytest.raises(ValueError):
         m(torch.tensor(1.0).half())
     assert len(entry_points) == seen
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("grad_mode", [False, True])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_a_tangent_is_not_dropped_by_the_gate(entry_points, which, grad_mode, requires_grad):
+    """There is no forward-mode formula: a tangent on any argument raises instead of giving a derivative of zero."""
+    args = [torch.zeros(3, 64), torch.zeros(16, 64), torch.zeros(16, 64), torch.zeros(16), torch.zeros(16)]
+    args = [t.half().requires_grad_(requires_grad) for t in args]
+    with torch.set_grad_enabled(grad_mode):
+        gated_linear(*args)
+        with forward_ad.dual_level():
+            gated_linear(*args)   # no tangent among them
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+            with pytest.raises(NotImplementedError):
+                gated_linear(*args)
+
+
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_a_tangent_is_not_dropped_by_the_gate_module(entry_points, grad_mode):
+    m = GatedLinear(64, 16, bias=True)
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(2, 3, 64).half(), torch.ones(2, 3, 64).half())
+        with pytest.raises(NotImplementedError):
+            m(x)

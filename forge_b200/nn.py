@@ -181,9 +181,36 @@ def _as_16bit_rows(x, features, dtype):
     return x.reshape(-1, x.shape[-1]).contiguous(), x.shape[:-1]
 
 
+def _has_tangent(tensors):
+    """Whether forward-mode differentiation is under way and one of `tensors` (or None) carries a tangent."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+class _InferenceOnlyFn(torch.autograd.Function):
+    """A call that has no derivative, kept in the graph so that a backward pass through it raises (as forward mode does, for
+    want of a formula) instead of ending there and leaving every gradient before it out."""
+
+    @staticmethod
+    def forward(ctx, call, *args):
+        return call(*args)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise NotImplementedError("4-bit layers are for inference only: no gradient passes through them")
+
+
+def _inference_only(call, x, *args):
+    """call(x, *args) for the tensors or None in `args`."""
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *args))) or _has_tangent((x, *args)):
+        return _InferenceOnlyFn.apply(call, x, *args)
+    return call(x, *args)
+
+
 class Int4Linear(nn.Module):
-    """Linear layer on 4-bit weights with one fp16 scale per `group_size` inputs; activations stay fp16 or bf16
-    (inference only). Built for few tokens, where its time is that of reading the weight; any number runs."""
+    """Linear layer on 4-bit weights with one fp16 scale per `group_size` inputs; activations stay fp16 or bf16. Inference
+    only: a backward pass through it raises, and its bias asks for no gradient. Built for few tokens, where its time is
+    that of reading the weight; any number runs."""
 
     def __init__(self, in_features, out_features, bias=True, group_size=128, dtype=torch.float16):
         super().__init__()
@@ -196,15 +223,18 @@ class Int4Linear(nn.Module):
         self.register_buffer("w_int4", torch.full((out_features, -(-in_features // 128) * 64), 0x88, dtype=torch.uint8))
         self.register_buffer("w_scale", torch.ones(-(-in_features // group_size), out_features, dtype=torch.float16))
         if bias:
-            self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype))
+            self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype), requires_grad=False)
         else:
             self.register_parameter("bias", None)
 
     def forward(self, x):
         x2, lead = _as_16bit_rows(x, self.in_features, self.dtype)
-        bias = None if self.bias is None else self.bias.detach().to(x2.dtype)
-        y = _C.int4_linear(x2.detach(), self.w_int4, self.w_scale, bias, self.group_size)
+        bias = None if self.bias is None else self.bias.to(x2.dtype)
+        y = _inference_only(self._run, x2, bias)
         return y.reshape(*lead, self.out_features)
+
+    def _run(self, x, bias):
+        return _C.int4_linear(x, self.w_int4, self.w_scale, bias, self.group_size)
 
     @torch.no_grad()
     def quantize_weight(self, weight_fp):
@@ -216,12 +246,6 @@ class Int4Linear(nn.Module):
     def extra_repr(self):
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.bias is not None}, group_size={self.group_size}")
-
-
-def _has_tangent(tensors):
-    """Whether forward-mode differentiation is under way and one of `tensors` (or None) carries a tangent."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _GatedLinearFn(torch.autograd.Function):
@@ -291,7 +315,8 @@ class GatedLinear(nn.Module):
 
 
 class Int4GatedLinear(nn.Module):
-    """SiLU(gate(x)) * up(x) on 4-bit weights, one kernel (inference only)."""
+    """SiLU(gate(x)) * up(x) on 4-bit weights, one kernel. Inference only: a backward pass through it raises, and its biases
+    ask for no gradient."""
 
     def __init__(self, in_features, out_features, bias=False, group_size=128, dtype=torch.float16):
         super().__init__()
@@ -307,16 +332,19 @@ class Int4GatedLinear(nn.Module):
             self.register_buffer(f"w_{k}_scale",
                                  torch.ones(-(-in_features // group_size), out_features, dtype=torch.float16))
             if bias:
-                self.register_parameter(f"b_{k}", nn.Parameter(torch.zeros(out_features, dtype=dtype)))
+                self.register_parameter(f"b_{k}", nn.Parameter(torch.zeros(out_features, dtype=dtype), requires_grad=False))
             else:
                 self.register_parameter(f"b_{k}", None)
 
     def forward(self, x):
         x2, lead = _as_16bit_rows(x, self.in_features, self.dtype)
-        bg, bu = (None if b is None else b.detach().to(x2.dtype) for b in (self.b_gate, self.b_up))
-        h = _C.int4_gated_linear(x2.detach(), self.w_gate_int4, self.w_up_int4, self.w_gate_scale, self.w_up_scale, bg, bu,
-                                 self.group_size)
+        bg, bu = (None if b is None else b.to(x2.dtype) for b in (self.b_gate, self.b_up))
+        h = _inference_only(self._run, x2, bg, bu)
         return h.reshape(*lead, self.out_features)
+
+    def _run(self, x, bg, bu):
+        return _C.int4_gated_linear(x, self.w_gate_int4, self.w_up_int4, self.w_gate_scale, self.w_up_scale, bg, bu,
+                                    self.group_size)
 
     @torch.no_grad()
     def quantize_weight(self, w_gate_fp, w_up_fp):

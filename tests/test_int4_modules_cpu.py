@@ -65,3 +65,41 @@ def test_a_tangent_is_not_dropped_by_the_gate_module(entry_points, grad_mode):
         x = forward_ad.make_dual(torch.zeros(2, 3, 64).half(), torch.ones(2, 3, 64).half())
         with pytest.raises(NotImplementedError):
             m(x)
+
+
+def _layers():
+    for make in (Int4Linear, Int4GatedLinear):
+        for bias in (False, True):
+            yield make(64, 16, bias=bias)
+
+
+def test_no_gradient_ends_silently_at_a_4_bit_layer(entry_points):
+    for m in _layers():
+        x = torch.zeros(2, 64).half()
+        assert not m(x).requires_grad           # nothing asks for a gradient: the parameters do not by default
+        y = m(x.requires_grad_())
+        assert y.requires_grad and y.shape == (2, 16)
+        with pytest.raises(NotImplementedError):
+            y.sum().backward()
+        with pytest.raises(NotImplementedError):   # converted on the way
+            m(torch.zeros(3, 2, 64, requires_grad=True)).sum().backward()
+        with torch.no_grad():
+            assert not m(x).requires_grad
+        with torch.inference_mode():
+            assert not m(x.detach()).requires_grad
+        assert all(not p.requires_grad for p in m.parameters())
+        for p in m.parameters():
+            p.requires_grad_()
+            with pytest.raises(NotImplementedError):
+                m(x.detach()).sum().backward()
+            p.requires_grad_(False)
+
+
+def test_a_tangent_is_not_dropped_by_a_4_bit_layer(entry_points):
+    for m in _layers():
+        for grad_mode in (False, True):
+            with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+                x = torch.zeros(2, 64).half()
+                m(x)
+                with pytest.raises(NotImplementedError):
+                    m(forward_ad.make_dual(x, torch.ones_like(x)))

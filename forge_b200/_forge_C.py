@@ -346,8 +346,8 @@ def gated_linear_backward(dh, x, Wg, Wu, g, u, need_x=True, need_w=True, need_b=
     _shape(dh=(dh, (M, N)), Wg=(Wg, (N, K)), Wu=(Wu, (N, K)), g=(g, (M, N)), u=(u, (M, N)))
     if N % 8 != 0 or N > _MAX_SIZE:
         raise ValueError(f"Wg, Wu: the number of outputs must be a multiple of 8, at most {_MAX_SIZE}, got {N}")
-    # without tokens the library writes nothing, and the gradients of the weights are zero
-    like = torch.zeros_like if M == 0 else torch.empty_like
+    # without tokens or outputs the library writes nothing: the gradients of the weights, or of x, are empty sums
+    like = torch.zeros_like if M == 0 or N == 0 else torch.empty_like
     dx = like(x) if need_x else None
     dWg, dWu = (like(Wg), like(Wu)) if need_w else (None, None)
     dbg = dbu = None

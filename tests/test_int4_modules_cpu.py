@@ -103,3 +103,17 @@ def test_a_tangent_is_not_dropped_by_a_4_bit_layer(entry_points):
                 m(x)
                 with pytest.raises(NotImplementedError):
                     m(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("M,N", [(0, 16), (3, 0), (0, 0)])
+def test_gradients_that_the_library_does_not_write_are_zero(monkeypatch, M, N):
+    """Without tokens or outputs an entry point returns at once; fresh memory may hold anything."""
+    monkeypatch.setattr(C, "_act_shape", lambda x: (1, *x.shape))
+    monkeypatch.setattr(C, "_chk", lambda *a, **k: None)
+    monkeypatch.setattr(C, "_run", lambda *a: None)
+    monkeypatch.setattr(torch, "empty_like", lambda t: torch.full_like(t, 7))
+    new = lambda *s: torch.zeros(*s).half()  # noqa: E731
+    saved = torch.zeros(M, N), torch.zeros(M, N)
+    grads = C.gated_linear_backward(new(M, N), new(M, 64), new(N, 64), new(N, 64), *saved)
+    assert [tuple(g.shape) for g in grads] == [(M, 64), (N, 64), (N, 64), (N,), (N,)]
+    assert all((g == 0).all() for g in grads)

@@ -30,12 +30,16 @@ from .nn import GatedLinear, Int4GatedLinear, Int4Linear, QuantizedLinear, Spars
 _SCHEMES = ("dynamic_int8", "static_int8", "weight_only_int8", "weight_only_int4")
 
 
-def _set_child(model, dotted, new_module):
+def _replace(model, dotted, new_module):
+    """`model` with its submodule `dotted` replaced; "" is the model itself, which is `new_module` then."""
+    if not dotted:
+        return new_module
     parent = model
     *path, leaf = dotted.split(".")
     for part in path:
         parent = getattr(parent, part)
     setattr(parent, leaf, new_module)
+    return model
 
 
 def _run_calibration(model, data, num_batches, forward_fn, device):
@@ -91,7 +95,8 @@ def quantize(model, calibration_data=None, num_calibration_batches=100, scheme="
     """Returns `model` with its `nn.Linear` layers replaced by W8A8 layers, or with scheme="weight_only_int4" (additive)
     by layers on 4-bit weights with one scale per `group_size` inputs: `nn.Linear` -> `Int4Linear` (layers with
     in_features % 8 != 0 become `QuantizedLinear`), `GatedLinear` -> `Int4GatedLinear`. The other schemes leave a
-    `GatedLinear` as it is.
+    `GatedLinear` as it is. A `model` that is itself such a layer comes back as the new layer, which inplace=True cannot do
+    (ValueError).
 
     Parameters up to `forward_fn` are the reference's (convert.py:19-26). Additive, keyword only:
     sparse=True prunes each weight 2:4 by magnitude and uses `SparseLinear` where the layer is on a
@@ -103,15 +108,18 @@ def quantize(model, calibration_data=None, num_calibration_batches=100, scheme="
     int4 = scheme == "weight_only_int4"
     if int4 and sparse:
         raise ValueError("sparse=True is for the INT8 schemes")
+    layers = (nn.Linear, GatedLinear) if int4 else nn.Linear
+    if inplace and isinstance(model, layers):
+        raise ValueError(f"a {type(model).__name__} cannot become another layer in place")
     if not inplace:
         model = copy.deepcopy(model)
     if int4:
         swaps = [(name, _to_int4(m, group_size) if m.in_features % 8 == 0 else _to_w8a8(m, False))
-                 for name, m in model.named_modules() if isinstance(m, (nn.Linear, GatedLinear))]
+                 for name, m in model.named_modules() if isinstance(m, layers)]
     else:
-        swaps = [(name, _to_w8a8(m, sparse)) for name, m in model.named_modules() if isinstance(m, nn.Linear)]
+        swaps = [(name, _to_w8a8(m, sparse)) for name, m in model.named_modules() if isinstance(m, layers)]
     for name, new in swaps:
-        _set_child(model, name, new)
+        model = _replace(model, name, new)
     if scheme == "static_int8" and calibration_data is not None:
         first = next(model.parameters(), None)
         device = first.device if first is not None else torch.device("cpu")
@@ -134,7 +142,7 @@ def finalize_qat(model, *, sparse=False, verbose=True):
     weights (convert.py:205-237). Additive: sparse=True as in `quantize`."""
     swaps = [(name, _to_w8a8(m.linear, sparse)) for name, m in model.named_modules() if _is_qat_wrapper(m)]
     for name, new in swaps:
-        _set_child(model, name, new)
+        model = _replace(model, name, new)
     if verbose:
         print(f"forge_b200.quant: finalized {len(swaps)} QAT layers")
     return model

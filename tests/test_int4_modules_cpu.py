@@ -2,10 +2,12 @@
 with the entry points replaced by stand-ins where a call would reach them."""
 import pytest
 import torch
+import torch.nn as nn
 from torch.autograd import forward_ad
 
 from forge_b200 import _forge_C as C
-from forge_b200.nn import GatedLinear, Int4GatedLinear, Int4Linear, gated_linear
+from forge_b200.nn import GatedLinear, Int4GatedLinear, Int4Linear, QuantizedLinear, gated_linear
+from forge_b200.quant import finalize_qat, quantize
 
 
 @pytest.fixture
@@ -117,3 +119,21 @@ def test_gradients_that_the_library_does_not_write_are_zero(monkeypatch, M, N):
     grads = C.gated_linear_backward(new(M, N), new(M, 64), new(N, 64), new(N, 64), *saved)
     assert [tuple(g.shape) for g in grads] == [(M, 64), (N, 64), (N, 64), (N,), (N,)]
     assert all((g == 0).all() for g in grads)
+
+
+def test_a_model_that_is_a_single_layer_is_converted():
+    for layer, scheme, want in ((nn.Linear(64, 24), "weight_only_int4", Int4Linear),
+                                (GatedLinear(64, 24, bias=True), "weight_only_int4", Int4GatedLinear),
+                                (nn.Linear(20, 24), "weight_only_int4", QuantizedLinear),
+                                (nn.Linear(64, 24), "dynamic_int8", QuantizedLinear)):
+        out = quantize(layer, scheme=scheme, verbose=False)
+        assert type(out) is want and out.out_features == 24
+        assert not list(layer.children()) and not list(out.children())
+        with pytest.raises(ValueError):   # the caller's object cannot change its class
+            quantize(layer, scheme=scheme, inplace=True, verbose=False)
+        assert not list(layer.children())
+    gate = GatedLinear(64, 24)
+    assert quantize(gate, inplace=True, verbose=False) is gate   # which the INT8 schemes leave as it is
+    wrapper = nn.Module()
+    wrapper.linear, wrapper.weight_fq, wrapper.input_fq = nn.Linear(64, 24), nn.Identity(), nn.Identity()
+    assert type(finalize_qat(wrapper, verbose=False)) is QuantizedLinear

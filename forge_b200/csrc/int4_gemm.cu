@@ -77,11 +77,14 @@ __device__ __forceinline__ void unpack_q(uint32_t w, __half2 (&q)[4]) {
                                __half2half2(__ushort_as_half(0xD480)));   // / 16 - 72
     }
 }
+// SHIFT: q 2^-SHIFT
+template <int SHIFT = 0>
 __device__ __forceinline__ void unpack_q(uint32_t w, __nv_bfloat162 (&q)[4]) {
+    constexpr uint32_t kOffset = 0x4300 - (SHIFT << 7), kOffset8 = kOffset + 8;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
-        q[i] = __hsub2(reinterpret_cast<const __nv_bfloat162&>(b), __bfloat162bfloat162(__ushort_as_bfloat16(0x4308)));
+        const uint32_t b = and_or(w >> (4 * i), 0x000F000Fu, kOffset * 0x10001u);
+        q[i] = __hsub2(reinterpret_cast<const __nv_bfloat162&>(b), __bfloat162bfloat162(__ushort_as_bfloat16(kOffset8)));
     }
 }
 template <typename V>
@@ -485,6 +488,9 @@ constexpr int kFirstSum = 3;              // warps: TMA, two MMA issuers, sums, 
 constexpr int kFirstWeight = kFirstSum + kSumWarps;
 constexpr int kTokenThreads = 32 * (kFirstWeight + kTokenRing * kTokenGroupWarps);
 constexpr int kSwapBytes = 32 * 64 * 4;   // gated: the up products of 32 tokens x 64 rows
+// bf16: the integers are multiplied as q 2^-11, so that a group's sum, 128 * 8 of the largest activation at most, stays
+// below it: no sum overflows before the scale is applied, whatever the activations are.
+constexpr int kShift = 11;
 __device__ __forceinline__ TokenBars carve_tokens(uint8_t* p) {
     TokenBars b;
     b.full_w = reinterpret_cast<uint64_t*>(p);
@@ -680,7 +686,8 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             typename std::conditional<BF16, __nv_bfloat162, __half2>::type q[4];
-                            unpack_q(word[j], q);
+                            if constexpr (BF16) unpack_q<kShift>(word[j], q);
+                            else unpack_q(word[j], q);
                             *reinterpret_cast<uint4*>(dst + (j / 2) * kSlab + i * (STEP * 128) +
                                                       (((4 * (j % 2) + t4) ^ row8) << 4)) = bits4(q);
                         }
@@ -732,7 +739,7 @@ int4_tokens_kernel(const __grid_constant__ CUtensorMap tm_x, const uint8_t* __re
                     constexpr int CHUNK = SUMS == 32 ? 32 : 16;   // columns at a time, as the registers allow
 #pragma unroll
                     for (int k = 0; k < SET; k++) {
-                        const float s = __half2float(__ushort_as_half(scales[h * SET + k]));
+                        const float s = __half2float(__ushort_as_half(scales[h * SET + k])) * (BF16 ? 1 << kShift : 1);
 #pragma unroll
                         for (int c = 0; c < SUMS / CHUNK; c++) {
                             // columns past `width` may hold anything: theirs are sums that nobody takes

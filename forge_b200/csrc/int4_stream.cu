@@ -44,7 +44,9 @@ constexpr int kTokStride = 20;        // floats per token of a partial sum: 16 r
 // pairs of 16-bit floats, the first two for one accumulator (A), the others for another (B); their sum is A + B * kB.
 //   fp16: a nibble alone in a half is the subnormal number n 2^-24, or 16 n 2^-24 where it lies four bits up; tensor
 //         cores take subnormals as they are. The factor 2^24 comes in behind the last sum.
-//   bf16: its subnormals would make subnormal fp32 products, so the nibble becomes the upper mantissa bits of 16 + n.
+//   bf16: its subnormals would make subnormal fp32 products, so the nibble becomes the upper mantissa bits of (16 + n) 2^-12:
+//         the most that a sum over a group can be is 128 * 31 * 2^-12 < 1 times the largest activation, so none overflows,
+//         whatever the activations are.
 template <typename T>
 struct Nibbles;
 template <>
@@ -61,13 +63,13 @@ struct Nibbles<__half> {
 };
 template <>
 struct Nibbles<__nv_bfloat16> {
-    static constexpr float kB = 1.f, kFactor = 1.f;
-    static constexpr uint32_t kMinusOffsetA = 0xC1C0C1C0u, kMinusOffsetB = 0xC1C0C1C0u;   // -24
+    static constexpr float kB = 1.f, kFactor = 4096.f;
+    static constexpr uint32_t kMinusOffsetA = 0xBBC0BBC0u, kMinusOffsetB = 0xBBC0BBC0u;   // -24 2^-12
     static __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&f)[4]) {
-        f[0] = and_or(w * 8u, 0x00780078u, 0x41804180u);
-        f[1] = and_or(w >> 1, 0x00780078u, 0x41804180u);
-        f[2] = and_or(w >> 5, 0x00780078u, 0x41804180u);
-        f[3] = and_or(w >> 9, 0x00780078u, 0x41804180u);
+        f[0] = and_or(w * 8u, 0x00780078u, 0x3B803B80u);
+        f[1] = and_or(w >> 1, 0x00780078u, 0x3B803B80u);
+        f[2] = and_or(w >> 5, 0x00780078u, 0x3B803B80u);
+        f[3] = and_or(w >> 9, 0x00780078u, 0x3B803B80u);
     }
 };
 

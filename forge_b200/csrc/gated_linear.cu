@@ -17,13 +17,16 @@
 // lie ("MN-major": 64 channels x 8 inputs per swizzle atom), so nothing is ever transposed in memory.
 //
 // 8192 tokens, 4096 -> 14336, bf16: forward 1.20 ms (1600 TFLOP/s, the burst rate of the tensor pipe), with g and u saved
-// 1.31 ms; backward 2.8-3.0 ms, of which the elementwise part takes 265 us and the products the rest (1500 TFLOP/s). 1001
-// tokens, 1032 -> 2744: forward 25 us, backward 64 us, with tens of tiles for 74 pairs; a step through autograd takes
-// 155 us of host time.
+// 1.31 ms; backward 2.7-3.0 ms, of which the elementwise part takes 265 us and the products the rest (1500 TFLOP/s), and
+// in fp16 0.15-0.19 ms more (see Precision). 1001 tokens, 1032 -> 2744: forward 25 us, backward 64 us (fp16 69), with tens of tiles
+// for 74 pairs; a step through autograd takes 155 us of host time.
 //
 // Precision: the forward keeps g and u in fp32 for the backward - 8 bytes per element, where rounding them to 16 bits
 // would put another two roundings into every gradient. dg and du are rounded to 16 bits, which the tensor cores
-// need; the bias gradients are summed from them before that rounding, in fp32, in a fixed order.
+// need; the bias gradients are summed from them before that rounding, in fp32, in a fixed order. Gradients are often so
+// small (or, with a scaled loss, so large) that fp16 would flush or overflow them although their products are in its
+// range: fp16 calls go through them once more beforehand for their largest value, store them times the power of two that
+// puts it into [2^14, 2^15), and take that off the fp32 sums. What lies 2^29 below the largest is still rounded to 11 bits.
 #include <algorithm>
 
 #include "common.cuh"
@@ -50,11 +53,12 @@ struct Maps {
 };
 
 // Rows (256 per tile) are tokens, or channels for kDw; columns are channels (kForward*: 128 per tile) or inputs.
-// rows, cols: extent of one output matrix; kb1: K blocks of the first operand pair, kbs: of both.
+// rows, cols: extent of one output matrix; kb1: K blocks of the first operand pair, kbs: of both. unscale (kDx and kDw, fp16):
+// what the products are multiplied by.
 template <int MODE, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 gated_pair_kernel(const __grid_constant__ Maps maps, const void* __restrict__ bias_g, const void* __restrict__ bias_u,
-                  int rows, int cols, int kb1, int kbs, int* __restrict__ status) {
+                  int rows, int cols, int kb1, int kbs, const float* __restrict__ unscale, int* __restrict__ status) {
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     constexpr bool FWD = MODE == kForward || MODE == kForwardSave;
     constexpr bool A_MN = MODE == kDw, B_MN = !FWD;
@@ -195,6 +199,8 @@ gated_pair_kernel(const __grid_constant__ Maps maps, const void* __restrict__ bi
         const int epi_tid = (warp_id - 2) * 32 + lane;
         uint8_t* my_stage = smem_epi + (warp_id - 2) * Cfg::kEpiBufs * Cfg::kEpiBufBytes;
         const uint64_t policy = l2_policy_evict_first();   // outputs must not push operands out of L2
+        constexpr bool SCALED = !FWD && !BF16;
+        const float factor = SCALED ? *unscale : 1.f;
         int sbuf = 0, local = 0;
         bool ok = true;
         // 32 rows x 128 bytes from this lane's 32 words, through a staging buffer, to column x, row y of `m`
@@ -267,7 +273,8 @@ gated_pair_kernel(const __grid_constant__ Maps maps, const void* __restrict__ bi
 #pragma unroll
                         for (int i = 0; i < 16; i++)
                             packed[hh * 16 + i] =
-                                pack2<T>(__uint_as_float(va[2 * i]), __uint_as_float(va[2 * i + 1]));
+                                SCALED ? pack2<T>(__uint_as_float(va[2 * i]) * factor, __uint_as_float(va[2 * i + 1]) * factor)
+                                       : pack2<T>(__uint_as_float(va[2 * i]), __uint_as_float(va[2 * i + 1]));
                     }
                 }
                 if (row0 < rows && n0 + c * 64 < cols) store(&maps.out[half], packed, n0 + c * 64, row0);
@@ -296,57 +303,134 @@ gated_pair_kernel(const __grid_constant__ Maps maps, const void* __restrict__ bi
 // ---------------------------------------------------------------------- elementwise part of the backward pass
 
 constexpr int kGateRows = 64;   // tokens per CTA
+constexpr int kMaxima = 1000;   // CTAs that look for the largest gradient, at most
+
+// dg and du of an element
+__device__ __forceinline__ float2 gate_gradients(float dh, float g, float u) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    return make_float2(dh * u * s * (1.f + g * (1.f - s)), dh * g * s);
+}
+
+template <typename T>
+struct Loaded {   // 8 neighbouring elements
+    uint4 d;
+    float4 g[2], u[2];
+    __device__ __forceinline__ float2 gradients(int i) const {
+        const float4 a = g[i / 4], b = u[i / 4];
+        const int e = i % 4;
+        return gate_gradients(to_float(reinterpret_cast<const T*>(&d)[i]), e == 0 ? a.x : e == 1 ? a.y : e == 2 ? a.z : a.w,
+                              e == 0 ? b.x : e == 1 ? b.y : e == 2 ? b.z : b.w);
+    }
+};
+
+__device__ __forceinline__ float block_max(float v) {   // of 256 threads, for all of them
+    __shared__ float warp_max[8];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = warp_max[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) v = fmaxf(v, warp_max[i]);
+    return v;
+}
+
+// maxima[CTA] = the largest finite |dg| or |du| of the CTA's share of `pieces` of 8 elements. Bound by HBM (10 bytes an
+// element). From the end to the beginning, where gate_backward_kernel starts: what is read last it finds in L2.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gate_maxima_kernel(const T* __restrict__ dh, const float* __restrict__ gate, const float* __restrict__ up,
+                   float* __restrict__ maxima, long long pieces) {
+    float most = 0.f;
+    const long long step = (long long)gridDim.x * 256;
+    for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < pieces; p += 2 * step) {
+        const bool two = p + step < pieces;   // two at a time, so that 160 bytes a thread are under way
+        Loaded<T> v[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (k == 0 || two) {
+                const long long at = pieces - 1 - (p + k * step);
+                v[k].d = __ldg(reinterpret_cast<const uint4*>(dh) + at);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    v[k].g[h] = __ldg(reinterpret_cast<const float4*>(gate) + 2 * at + h);
+                    v[k].u[h] = __ldg(reinterpret_cast<const float4*>(up) + 2 * at + h);
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (k == 0 || two) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 d = v[k].gradients(i);
+                    const float a = fabsf(d.x), b = fabsf(d.y);
+                    if (a < __int_as_float(0x7f800000)) most = fmaxf(most, a);   // infinities and NaNs stay what they are
+                    if (b < __int_as_float(0x7f800000)) most = fmaxf(most, b);
+                }
+            }
+    }
+    most = block_max(most);
+    if (threadIdx.x == 0) maxima[blockIdx.x] = most;
+}
 
 // A CTA takes 256 channels x kGateRows tokens: 32 threads across (8 channels each), 8 down. Bound by HBM (14 bytes an
-// element). BIAS: per-CTA column sums into part (2, row chunks, N), reduced by sum_parts_kernel.
+// element). BIAS: per-CTA column sums into part (2, row chunks, N), reduced by sum_parts_kernel. fp16: dg and du are stored
+// times the power of two that the maxima ask for, whose inverse goes to `unscale`.
 template <typename T, bool BIAS>
 __global__ void __launch_bounds__(256)
 gate_backward_kernel(const T* __restrict__ dh, const float* __restrict__ gate, const float* __restrict__ up,
-                     T* __restrict__ dg, T* __restrict__ du, float* __restrict__ part, int M, int N) {
+                     T* __restrict__ dg, T* __restrict__ du, float* __restrict__ part, const float* __restrict__ maxima,
+                     int num_maxima, float* __restrict__ unscale, int M, int N) {
+    constexpr bool SCALED = std::is_same<T, __half>::value;
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int n = (blockIdx.x * 32 + tx) * 8;
     const long long m0 = (long long)blockIdx.y * kGateRows;
+    float scale = 1.f;
+    if constexpr (SCALED) {
+        float most = 0.f;
+        for (int i = threadIdx.x; i < num_maxima; i += 256) most = fmaxf(most, maxima[i]);
+        most = block_max(most);
+        // both powers stay normal numbers
+        const int e = most > 0.f ? min(14 - ((int)(__float_as_uint(most) >> 23) - 127), 126) : 0;
+        scale = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *unscale = __uint_as_float((uint32_t)(127 - e) << 23);
+    }
     float sg[8] = {}, su[8] = {};
     if (n < N) {
         // two rows at a time, so that 160 bytes a thread are under way
         for (int r0 = ty; r0 < kGateRows && m0 + r0 < M; r0 += 16) {
             const bool two = r0 + 8 < kGateRows && m0 + r0 + 8 < M;
-            uint4 d4[2];
-            float4 g4[2][2], u4[2][2];
+            Loaded<T> v[2];
 #pragma unroll
             for (int k = 0; k < 2; k++)
                 if (k == 0 || two) {
                     const size_t at = (size_t)(m0 + r0 + 8 * k) * N + n;
-                    d4[k] = __ldcs(reinterpret_cast<const uint4*>(dh + at));
+                    v[k].d = __ldcs(reinterpret_cast<const uint4*>(dh + at));
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        g4[k][h] = __ldcs(reinterpret_cast<const float4*>(gate + at) + h);
-                        u4[k][h] = __ldcs(reinterpret_cast<const float4*>(up + at) + h);
+                        v[k].g[h] = __ldcs(reinterpret_cast<const float4*>(gate + at) + h);
+                        v[k].u[h] = __ldcs(reinterpret_cast<const float4*>(up + at) + h);
                     }
                 }
 #pragma unroll
             for (int k = 0; k < 2; k++)
                 if (k == 0 || two) {
                     const size_t at = (size_t)(m0 + r0 + 8 * k) * N + n;
-                    const T* d = reinterpret_cast<const T*>(&d4[k]);
-                    float g[8] = {g4[k][0].x, g4[k][0].y, g4[k][0].z, g4[k][0].w, g4[k][1].x, g4[k][1].y, g4[k][1].z, g4[k][1].w};
-                    float u[8] = {u4[k][0].x, u4[k][0].y, u4[k][0].z, u4[k][0].w, u4[k][1].x, u4[k][1].y, u4[k][1].z, u4[k][1].w};
+                    float a[8], b[8];
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float s = __fdividef(1.f, 1.f + __expf(-g[i]));
-                        const float v = to_float(d[i]);
-                        const float a = v * u[i] * s * (1.f + g[i] * (1.f - s)), b = v * g[i] * s;
-                        g[i] = a;
-                        u[i] = b;
+                        const float2 d = v[k].gradients(i);
                         if (BIAS) {
-                            sg[i] += a;
-                            su[i] += b;
+                            sg[i] += d.x;
+                            su[i] += d.y;
                         }
+                        a[i] = SCALED ? d.x * scale : d.x;
+                        b[i] = SCALED ? d.y * scale : d.y;
                     }
-                    *reinterpret_cast<uint4*>(dg + at) = make_uint4(pack2<T>(g[0], g[1]), pack2<T>(g[2], g[3]),
-                                                                    pack2<T>(g[4], g[5]), pack2<T>(g[6], g[7]));
-                    *reinterpret_cast<uint4*>(du + at) = make_uint4(pack2<T>(u[0], u[1]), pack2<T>(u[2], u[3]),
-                                                                    pack2<T>(u[4], u[5]), pack2<T>(u[6], u[7]));
+                    *reinterpret_cast<uint4*>(dg + at) = make_uint4(pack2<T>(a[0], a[1]), pack2<T>(a[2], a[3]),
+                                                                    pack2<T>(a[4], a[5]), pack2<T>(a[6], a[7]));
+                    *reinterpret_cast<uint4*>(du + at) = make_uint4(pack2<T>(b[0], b[1]), pack2<T>(b[2], b[3]),
+                                                                    pack2<T>(b[4], b[5]), pack2<T>(b[6], b[7]));
                 }
         }
     }
@@ -397,33 +481,40 @@ sum_parts_kernel(const float* __restrict__ part, T* __restrict__ dbg, T* __restr
 
 template <int MODE, bool BF16>
 int launch_pair(const Maps& maps, const void* bg, const void* bu, int rows, int cols, int kb1, int kbs,
-                cudaStream_t stream) {
+                const float* unscale, cudaStream_t stream) {
     static int max_pairs[64] = {};
     constexpr int TILE_N = MODE <= kForwardSave ? 128 : 256;
     const long long tiles = ((long long)rows + 255) / 256 * (MODE == kDw ? 2 : 1) * (((long long)cols + TILE_N - 1) / TILE_N);
     int* status = status_word();
     if (status == nullptr) return kLaunchFailed;
     return launch_pairs16(gated_pair_kernel<MODE, BF16>, kThreads, tiles, stream, max_pairs, maps, bg, bu, rows, cols, kb1,
-                          kbs, status);
+                          kbs, unscale, status);
 }
 
 inline size_t pad256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 inline int row_chunks(int M) { return (M + kGateRows - 1) / kGateRows; }
 
 template <typename T>
-int gate_backward(const void* dh, const float* g, const float* u, void* dg, void* du, float* part, void* dbg, void* dbu,
-                  int M, int N, cudaStream_t stream) {
+int gate_backward(const void* dh, const float* g, const float* u, void* dg, void* du, float* part, float* maxima,
+                  float* unscale, void* dbg, void* dbu, int M, int N, cudaStream_t stream) {
     const dim3 grid((N + 255) / 256, row_chunks(M), 1);
     if (grid.y > 65535) return kTooLarge;
     const T* d = static_cast<const T*>(dh);
     T *a = static_cast<T*>(dg), *b = static_cast<T*>(du);
+    int num_maxima = 0;
+    if (std::is_same<T, __half>::value) {
+        const long long pieces = (long long)M * N / 8;
+        num_maxima = (int)std::min<long long>((pieces + 511) / 512, std::min(4 * sm_count(), kMaxima));
+        gate_maxima_kernel<T><<<num_maxima, 256, 0, stream>>>(d, g, u, maxima, pieces);
+        if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
+    }
     if (dbg != nullptr || dbu != nullptr) {
-        gate_backward_kernel<T, true><<<grid, 256, 0, stream>>>(d, g, u, a, b, part, M, N);
+        gate_backward_kernel<T, true><<<grid, 256, 0, stream>>>(d, g, u, a, b, part, maxima, num_maxima, unscale, M, N);
         if (cudaGetLastError() != cudaSuccess) return kLaunchFailed;
         sum_parts_kernel<T><<<dim3((N + 31) / 32, 2, 1), 256, 0, stream>>>(part, static_cast<T*>(dbg), static_cast<T*>(dbu),
                                                                           (int)grid.y, N);
     } else {
-        gate_backward_kernel<T, false><<<grid, 256, 0, stream>>>(d, g, u, a, b, part, M, N);
+        gate_backward_kernel<T, false><<<grid, 256, 0, stream>>>(d, g, u, a, b, part, maxima, num_maxima, unscale, M, N);
     }
     return cudaGetLastError() == cudaSuccess ? kOk : kLaunchFailed;
 }
@@ -444,14 +535,15 @@ int gated_linear(const void* x, const void* wg, const void* wu, const void* bg, 
         return kLaunchFailed;
     const int kbs = (K + 63) / 64;
     if (g != nullptr)
-        return bf16 ? launch_pair<kForwardSave, true>(m, bg, bu, M, N, kbs, kbs, stream)
-                    : launch_pair<kForwardSave, false>(m, bg, bu, M, N, kbs, kbs, stream);
-    return bf16 ? launch_pair<kForward, true>(m, bg, bu, M, N, kbs, kbs, stream)
-                : launch_pair<kForward, false>(m, bg, bu, M, N, kbs, kbs, stream);
+        return bf16 ? launch_pair<kForwardSave, true>(m, bg, bu, M, N, kbs, kbs, nullptr, stream)
+                    : launch_pair<kForwardSave, false>(m, bg, bu, M, N, kbs, kbs, nullptr, stream);
+    return bf16 ? launch_pair<kForward, true>(m, bg, bu, M, N, kbs, kbs, nullptr, stream)
+                : launch_pair<kForward, false>(m, bg, bu, M, N, kbs, kbs, nullptr, stream);
 }
 
 size_t gated_linear_backward_workspace(int M, int N) {
-    return 2 * pad256((size_t)M * N * 2) + pad256((size_t)2 * row_chunks(M) * N * sizeof(float));
+    return 2 * pad256((size_t)M * N * 2) + pad256((size_t)2 * row_chunks(M) * N * sizeof(float)) +
+           pad256((kMaxima + 1) * sizeof(float));
 }
 
 int gated_linear_backward(const void* dh, const void* x, const void* wg, const void* wu, const float* g, const float* u,
@@ -461,8 +553,10 @@ int gated_linear_backward(const void* dh, const void* x, const void* wg, const v
     void* dg = ws;
     void* du = ws + pad256((size_t)M * N * 2);
     float* part = reinterpret_cast<float*>(ws + 2 * pad256((size_t)M * N * 2));
-    int r = bf16 ? gate_backward<__nv_bfloat16>(dh, g, u, dg, du, part, dbg, dbu, M, N, stream)
-                 : gate_backward<__half>(dh, g, u, dg, du, part, dbg, dbu, M, N, stream);
+    float* unscale = part + pad256((size_t)2 * row_chunks(M) * N * sizeof(float)) / sizeof(float);
+    float* maxima = unscale + 1;
+    int r = bf16 ? gate_backward<__nv_bfloat16>(dh, g, u, dg, du, part, maxima, unscale, dbg, dbu, M, N, stream)
+                 : gate_backward<__half>(dh, g, u, dg, du, part, maxima, unscale, dbg, dbu, M, N, stream);
     if (r != kOk) return r;
     const CUtensorMapDataType t = type16(bf16);
     if (dx != nullptr) {
@@ -472,8 +566,8 @@ int gated_linear_backward(const void* dh, const void* x, const void* wg, const v
             !encode_sw128(&m.out[0], t, 2, dx, K, M, 32))
             return kLaunchFailed;
         const int kb = (N + 63) / 64;
-        r = bf16 ? launch_pair<kDx, true>(m, nullptr, nullptr, M, K, kb, 2 * kb, stream)
-                 : launch_pair<kDx, false>(m, nullptr, nullptr, M, K, kb, 2 * kb, stream);
+        r = bf16 ? launch_pair<kDx, true>(m, nullptr, nullptr, M, K, kb, 2 * kb, unscale, stream)
+                 : launch_pair<kDx, false>(m, nullptr, nullptr, M, K, kb, 2 * kb, unscale, stream);
         if (r != kOk) return r;
     }
     if (dwg != nullptr) {
@@ -483,8 +577,8 @@ int gated_linear_backward(const void* dh, const void* x, const void* wg, const v
             !encode_sw128(&m.out[1], t, 2, dwu, K, N, 32))
             return kLaunchFailed;
         const int kb = (M + 63) / 64;
-        r = bf16 ? launch_pair<kDw, true>(m, nullptr, nullptr, N, K, kb, kb, stream)
-                 : launch_pair<kDw, false>(m, nullptr, nullptr, N, K, kb, kb, stream);
+        r = bf16 ? launch_pair<kDw, true>(m, nullptr, nullptr, N, K, kb, kb, unscale, stream)
+                 : launch_pair<kDw, false>(m, nullptr, nullptr, N, K, kb, kb, unscale, stream);
     }
     return r;
 }

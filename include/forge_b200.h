@@ -222,7 +222,9 @@ int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void
 
 /* Its gradients for dh (M,N): dx (M,K), dWg / dWu (N,K, both or neither NULL), dbg / dbu (N), each NULL when not wanted,
  * all of `dtype`; g and u as the forward call wrote them. The gradients of g and u are rounded to `dtype` before the
- * products, everything else is fp32; the order of every sum is fixed. `workspace` is caller-owned device memory of
+ * products, everything else is fp32; the order of every sum is fixed. fp16: they are first multiplied by the power of two
+ * that puts the call's largest finite one into [2^14, 2^15), which is taken off the sums, so they neither overflow nor,
+ * down to 2^-29 of the largest, lose bits. `workspace` is caller-owned device memory of
  * forge_gated_linear_backward_workspace_bytes(M, N) bytes, 256-byte aligned. With M <= 0 or N <= 0 nothing is
  * written, although the gradients of the weights, or of x, are then zero. At most 4194240 tokens (FORGE_B200_TOO_LARGE otherwise). */
 unsigned long long forge_gated_linear_backward_workspace_bytes(int M, int N);

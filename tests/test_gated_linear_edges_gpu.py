@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import float_ref as R
 from forge_b200 import _forge_C as C
 from forge_b200.nn import GatedLinear, gated_linear
 
@@ -23,3 +24,90 @@ def test_no_outputs():
         assert m.w_gate.grad.shape == (0, 64) and m.b_up.grad.shape == (0,)
     torch.cuda.synchronize()
     assert C.device_status() == 0
+
+
+def _gradients(dh, x, wg, wu):
+    """{name: (value, bound)} in 64 bits for fp16 calls without biases. dg and du are rounded to 11 bits, or where one lies
+    more than 2^29 below the call's largest, in steps of 2^-24 of the power of two below 2^-14 of the latter: half of one
+    is at most 2^-39 of the largest. The other terms are those of float_ref.gate_backward."""
+    g, eg, u, eu = R.gate(x, wg, wu, None, None)[2]
+    dh, x, wg, wu = (t.double() for t in (dh, x, wg, wu))
+    s = torch.sigmoid(g)
+    dg, du = dh * u * s * (1 + g * (1 - s)), dh * g * s
+    eg, eu = (dh.abs() * (1.1 * eu + 0.5 * eg * (u.abs() + eu))
+              + R._fn_rel(g) * 2 * (dh * u * s).abs() * (1 + (g * (1 - s)).abs()) + 2.0 ** -120,
+              dh.abs() * 1.1 * eg + R._fn_rel(g) * du.abs() + 2.0 ** -120)
+    finite = lambda t: t.nan_to_num(0, 0, 0)  # noqa: E731
+    floor = 2.0 ** -39 * torch.maximum(finite(dg.abs() + eg).max(), finite(du.abs() + eu).max())
+    rg, ru = (e + (d.abs() + e) * 2.0 ** -11 + floor for d, e in ((dg, eg), (du, eu)))
+    (M, N), acc = dh.shape, 2.0 ** -23
+    a, b = dg.abs() + rg, du.abs() + ru
+    out = {
+        "dx": (dg @ wg + du @ wu, rg @ wg.abs() + ru @ wu.abs() + (2 * N + 64) * acc * (a @ wg.abs() + b @ wu.abs())),
+        "dwg": (dg.t() @ x, rg.t() @ x.abs() + (M + 64) * acc * (a.t() @ x.abs())),
+        "dwu": (du.t() @ x, ru.t() @ x.abs() + (M + 64) * acc * (b.t() @ x.abs())),
+    }
+    return {k: (v, e + R.half_step(v.abs() + e, torch.float16)) for k, (v, e) in out.items()}
+
+
+def _fp16_case(M, K, N, seed, x_size, wg_size, wu_size):
+    gen = torch.Generator().manual_seed(seed)
+    new = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, wg, wu, dh = new(M, K) * x_size, new(N, K) * wg_size, new(N, K) * wu_size, new(M, N)
+    return [t.half().to(DEV).requires_grad_() for t in (x, wg, wu)], dh.to(DEV)
+
+
+# gradients as they are behind a mean over many tokens, and as a scaled loss makes them; all subnormal in the last
+@pytest.mark.parametrize("size", [1e-2, 1e-4, 1e-5, 1e-6, 1e-7, 100.0, 3000.0])
+@pytest.mark.parametrize("M,K,N", [(64, 64, 72), (1000, 72, 264), (2048, 64, 64)])
+def test_gradients_of_any_size(M, K, N, size):
+    args, dh = _fp16_case(M, K, N, M, 0.3, 0.6 * K ** -0.5, 0.6 * K ** -0.5)
+    dh = (dh * size).half()
+    got = torch.autograd.grad(gated_linear(*args), args, dh)
+    with torch.no_grad():
+        want = _gradients(dh, *args)
+    for name, t in zip(want, got):
+        R.close(t, *want[name], name)
+
+
+def test_gradients_of_the_gate_beyond_fp16():
+    """dh u is up to half a million, the gradients of x and the weights are within fp16's range."""
+    args, dh = _fp16_case(48, 64, 64, 5, 2.0 ** -6, 2.0 ** -6, 1000.0)
+    dh = (dh * 700).half()
+    got = torch.autograd.grad(gated_linear(*args), args, dh)
+    with torch.no_grad():
+        x, wg, wu = args
+        assert (dh.double() * (x.double() @ wu.double().t())).abs().max() > 4 * 65504
+        want = _gradients(dh, *args)
+        assert all(v.abs().max() < 65504 for v, _ in want.values())
+    for name, t in zip(want, got):
+        assert t.isfinite().all()
+        R.close(t, *want[name], name)
+
+
+def test_gradients_of_tokens_far_apart_in_size():
+    """Token m's gradient is 2^-m of the first one's, down to 2^-24 (subnormal numbers themselves)."""
+    args, dh = _fp16_case(25, 64, 72, 7, 1.0, 0.125, 0.125)
+    dh = (dh * 2.0 ** -torch.arange(25.0, device=DEV)[:, None]).half()
+    got = torch.autograd.grad(gated_linear(*args), args, dh)
+    with torch.no_grad():
+        want = _gradients(dh, *args)
+    for name, t in zip(want, got):
+        R.close(t, *want[name], name)
+
+
+def test_no_gradient_and_infinite_gradients():
+    args, dh = _fp16_case(40, 64, 72, 9, 1.0, 0.125, 0.125)
+    dh = (dh * 1e-6).half()
+    h = gated_linear(*args)
+    assert all((t == 0).all() for t in torch.autograd.grad(h, args, torch.zeros_like(dh), retain_graph=True))
+    dh[3] = 0
+    want = torch.autograd.grad(h, args, dh, retain_graph=True)
+    for bad in (float("inf"), float("nan")):
+        dh[3, 70] = bad
+        dx, dwg, dwu = torch.autograd.grad(h, args, dh, retain_graph=True)
+        rows = [m for m in range(40) if m != 3]
+        outs = [n for n in range(72) if n != 70]
+        assert torch.equal(dx[rows], want[0][rows]) and not dx[3].isfinite().any()
+        assert torch.equal(dwg[outs], want[1][outs]) and torch.equal(dwu[outs], want[2][outs])
+        assert not dwg[70].isfinite().any() and not dwu[70].isfinite().any()

@@ -1,10 +1,17 @@
-"""The gated linear layer at the ends of its range: layers without outputs and gradients far from one in size."""
+"""The gated linear layer at the ends of its range (no outputs, gradients far from one in size), compiled, and called first
+from several threads."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
+import torch.nn as nn
 
 import float_ref as R
 from forge_b200 import _forge_C as C
 from forge_b200.nn import GatedLinear, gated_linear
+from forge_b200.quant import quantize
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -111,3 +118,66 @@ def test_no_gradient_and_infinite_gradients():
         assert torch.equal(dx[rows], want[0][rows]) and not dx[3].isfinite().any()
         assert torch.equal(dwg[outs], want[1][outs]) and torch.equal(dwu[outs], want[2][outs])
         assert not dwg[70].isfinite().any() and not dwu[70].isfinite().any()
+
+
+def test_a_compiled_block_is_the_block():
+    """Dynamo breaks its graph around the library's calls; results and gradients are those of the uncompiled module."""
+    torch.manual_seed(0)
+    block = nn.Sequential(nn.Linear(128, 64, device=DEV, dtype=torch.float16), GatedLinear(64, 264, bias=True, device=DEV),
+                          nn.Linear(264, 128, device=DEV, dtype=torch.float16))
+    x = torch.randn(3, 40, 128, device=DEV).half()
+
+    def step(f):
+        block.zero_grad()
+        y = f(x)
+        y.float().square().sum().backward()
+        return [y.detach(), *(p.grad for p in block.parameters())]
+    want = step(block)
+    torch._dynamo.reset()
+    fast = torch.compile(block, backend="eager")
+    assert all(torch.equal(a, b) for a, b in zip(step(fast), want))
+    served = quantize(block, scheme="weight_only_int4", group_size=32, verbose=False)
+    with torch.no_grad():
+        assert torch.equal(torch.compile(served, backend="eager")(x), served(x))
+    torch._dynamo.reset()
+
+
+_THREADS = """
+import sys, threading, torch
+sys.path.insert(0, sys.argv[1])
+from forge_b200 import _forge_C as C
+from forge_b200.nn import gated_linear
+def step(seed):
+    gen = torch.Generator().manual_seed(seed)
+    new = lambda *s: torch.randn(*s, generator=gen).half().cuda()
+    x, wg, wu, dh = new(40, 64), new(72, 64), new(72, 64), new(40, 72)
+    a = [t.requires_grad_() for t in (x, wg, wu)]
+    grads = torch.autograd.grad(gated_linear(*a), a, dh)
+    with torch.no_grad():
+        w, s = C.prepare_weight_int4(wg, 32)
+        few = C.int4_linear(x[:3], w, s, None, 32)
+        return [*grads, gated_linear(x[:3], wg, wu), few, C.int4_linear(x, w, s, None, 32),
+                C.int4_gated_linear(x[:3], w, w, s, s, None, None, 32)]
+start, got = threading.Barrier(4), [None] * 4
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        got[i] = step(i)
+        torch.cuda.current_stream().synchronize()
+torch.zeros(1, device="cuda")
+threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+for i in range(4):
+    assert all(torch.equal(a, b) for a, b in zip(got[i], step(i))), i
+torch.cuda.synchronize()
+assert C.device_status() == 0
+print("threads ok")
+"""
+
+
+def test_first_calls_of_several_threads():
+    """A process whose first calls come from four threads at once."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", _THREADS, root], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "threads ok" in run.stdout, run.stderr[-2000:]

@@ -137,3 +137,27 @@ def test_a_model_that_is_a_single_layer_is_converted():
     wrapper = nn.Module()
     wrapper.linear, wrapper.weight_fq, wrapper.input_fq = nn.Linear(64, 24), nn.Identity(), nn.Identity()
     assert type(finalize_qat(wrapper, verbose=False)) is QuantizedLinear
+
+
+def test_an_entry_point_runs_on_its_tensors_device_and_stream(monkeypatch):
+    """Tensors of GPU 1 while GPU 0 is current, and of the current one; without a GPU the device switch is a stand-in."""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+    state, calls = {"device": 0}, []
+
+    @contextmanager
+    def device(d):
+        before, state["device"] = state["device"], d.index
+        yield
+        state["device"] = before
+
+    def call(name, *args):
+        calls.append((name, state["device"], args))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["device"])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(C._lib, "call", call)
+    monkeypatch.setattr(C._lib, "load", lambda: SimpleNamespace(entry=lambda *a: call("entry", *a) or 0))
+    for index in (1, 0):
+        C._run(SimpleNamespace(device=SimpleNamespace(index=index)), "entry", 7, 8)
+    assert calls == [("entry", 1, (7, 8, 101)), ("entry", 0, (7, 8, 100))] and state["device"] == 0

@@ -1,4 +1,4 @@
-// Pieces shared by the kernels that take fp16 or bf16 activations (wstream.cu, int4.cu, gated_linear.cu).
+// Pieces shared by the kernels that take fp16 or bf16 activations (int4*.cu, gated_*.cu).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -18,8 +18,8 @@
 //
 // 8192 tokens, 4096 -> 14336, bf16: forward 1.20 ms (1600 TFLOP/s, the burst rate of the tensor pipe), with g and u saved
 // 1.31 ms; backward 2.7-3.0 ms, of which the elementwise part takes 265 us and the products the rest (1500 TFLOP/s), and
-// in fp16 0.15-0.19 ms more (see Precision). 1001 tokens, 1032 -> 2744: forward 25 us, backward 64 us (fp16 69), with tens of tiles
-// for 74 pairs; a step through autograd takes 155 us of host time.
+// in fp16 0.15-0.19 ms more (see Precision). 1001 tokens, 1032 -> 2744: forward 25 us, backward 64 us (fp16 69), with tens
+// of tiles for 74 pairs; a step through autograd takes 155-160 us of host time.
 //
 // Precision: the forward keeps g and u in fp32 for the backward - 8 bytes per element, where rounding them to 16 bits
 // would put another two roundings into every gradient. dg and du are rounded to 16 bits, which the tensor cores
@@ -502,7 +502,7 @@ int gate_backward(const void* dh, const float* g, const float* u, void* dg, void
     const T* d = static_cast<const T*>(dh);
     T *a = static_cast<T*>(dg), *b = static_cast<T*>(du);
     int num_maxima = 0;
-    if (std::is_same<T, __half>::value) {
+    if constexpr (std::is_same<T, __half>::value) {
         const long long pieces = (long long)M * N / 8;
         num_maxima = (int)std::min<long long>((pieces + 511) / 512, std::min(4 * sm_count(), kMaxima));
         gate_maxima_kernel<T><<<num_maxima, 256, 0, stream>>>(d, g, u, maxima, pieces);

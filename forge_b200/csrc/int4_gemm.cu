@@ -21,7 +21,9 @@
 // Beyond 128 tokens: 2048 x 4096 x 11008 142 us (1300 TFLOP/s, tensor pipe 71 % busy), 4096 x 4096 x 11008 285 us; gated,
 // 4096 -> 14336, 2048 tokens 705 us (74 %) and 8192 tokens 2.8-3.0 ms (1300 TFLOP/s, half of them the rest's). A block takes
 // 0.88 us where its tensor instructions take 0.55: a stage is refilled once they are done with it, and 192 KB are three.
-// Weights made in registers ahead of the stage do not help (156 us: the registers spill).
+// Weights made in registers ahead of the stage do not help (156 us: the registers spill; of what is here, 96 registers a
+// thread, the gated kernel spills 68 to 72 bytes, the plain one 8 to 32, the kernel for 17 to 128 tokens 102 to 136 with
+// 128 columns and up to 46 with fewer).
 // The kernel for 17 to 128 tokens is described below. It pays up to 128, apart from its sums: at 65 to 96 tokens 31 us
 // against 34 here with 11008 x 4096 and groups of 128 (with groups of 32 50), 45 against 95 with 4096 x 14336, gated 67
 // against 115; at 128 tokens 34 on both sides, 48 against 95 and 78 against 117.

@@ -21,7 +21,9 @@
 // Cold weights: 11008 x 4096 fp16, groups of 128, 9.7 us at 1 token and 10.6 at 8 (22.9 MB: 2.4 TB/s; 3.5 us at the copy
 // rate, an empty launch 2); 4096 x 14336 bf16, groups of 64, 14 and 15 us; 8192 x 8192 12 and 12.6; 28672 x 8192 32 us (3.7
 // TB/s); gated 14336 x 4096 twice 22 and 24 us (60.6 MB: 2.8 TB/s). 4096 x 14336: half of the issue slots are used and a
-// fifth of the memory's rate; what is left is latency, of the activations from L2 and of few blocks for each warp. 16
+// fifth of the memory's rate; what is left is latency, of the activations from L2 and of few blocks for each warp, and
+// registers: with two row blocks and groups of 32 or 64 every instance spills, 60 to 96 bytes of stores a thread with 80
+// registers (up to 8 tokens), 40 to 268 with 128; groups of 128 at most 36. 16
 // tokens need two products a fragment and the registers of 16 warps an SM: 17 us for the first.
 //
 // The order of the sums is fixed (blocks of a warp, warps of a CTA): results do not change from run to run. Rows past N

@@ -216,7 +216,8 @@ enum {
  * x (M,K), Wg / Wu (N,K), bg / bu (N, may be NULL), h (M,N), all of `dtype` (FORGE_DTYPE_F16 or _BF16). g_out / u_out:
  * (M,N) fp32 that receive g and u for the backward pass, both or neither NULL. Products, gate and sums are evaluated in
  * fp32, h is rounded once. Needs K % 8 == 0, N % 8 == 0, sizes up to 2^30 and 16-byte aligned matrices
- * (FORGE_B200_BAD_SHAPE otherwise). */
+ * (FORGE_B200_BAD_SHAPE otherwise). Here and below a call with a size <= 0 returns FORGE_B200_OK and writes nothing, with
+ * K <= 0 too. */
 int forge_gated_linear(const void* x, const void* Wg, const void* Wu, const void* bg, const void* bu, void* h,
                        float* g_out, float* u_out, int M, int K, int N, int dtype, forge_stream_t stream);
 
